@@ -356,6 +356,136 @@ typedef struct mskv_filter_desc {
 uint64_t mskv_image_filter_workspace_bytes(int32_t img_seq, int32_t text_seq);
 int mskv_image_filter(const mskv_filter_desc* d, void* stream);
 
+/* ---- 8-bit paged KV cache -------------------------------------------------------------------
+ * No counterpart in the reference (its cache is 16-bit and lives on the host): K and V of
+ * sequences that fit HBM at one byte per value, in pages of page_size tokens, with the block
+ * selection and the attention that read them.
+ *
+ * A value is code * 2^e: an 8-bit float (MSKV_DT_FP8_E4M3, largest finite code 448, or
+ * MSKV_DT_FP8_E5M2, 57344) and an int8 exponent per (page, KV head), one for K and one for V,
+ * in [MSKV_KV8_EXP_MIN, MSKV_KV8_EXP_MAX].
+ *   code (page, h, row, d) at k (v) + page*stride_page + h*stride_h + row*head_dim + d
+ *   exponent of K (i = 0) / V (i = 1) of (page, h) at exps[(page*kv_heads + h)*2 + i]
+ *   bounds: the elementwise minimum (i = 0) and maximum (i = 1) of the page's K codes, in the
+ *   same 8-bit type, at bounds + ((page*kv_heads + h)*2 + i)*head_dim + d
+ * Token t of sequence b is row t % page_size of page page_table[b*pt_stride_b + t/page_size].
+ * Requirements: page_size a multiple of 16, <= 128; head_dim 64, 128 or 256; k, v and bounds
+ * 16-byte aligned, stride_page and stride_h multiples of 16 bytes.                           */
+#define MSKV_KV8_EXP_MIN (-60)
+#define MSKV_KV8_EXP_MAX 60
+#define MSKV_KV8_MAX_QLEN 16
+typedef struct mskv_kv8_pages {
+  void* k;
+  void* v;
+  void* exps;
+  void* bounds;                 /* NULL: none (mskv_kv8_block_score needs them)       */
+  const int32_t* page_table;
+  int64_t stride_page;          /* bytes, k and v alike                               */
+  int64_t stride_h;
+  int64_t pt_stride_b;          /* elements                                           */
+  int64_t num_pages;            /* page ids must lie in [0, num_pages)                */
+  int32_t max_pages;            /* entries of a page-table row                        */
+  int32_t page_size;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t dtype;                /* MSKV_DT_FP8_E4M3 or MSKV_DT_FP8_E5M2               */
+  int32_t batch;
+} mskv_kv8_pages;
+
+/* Append.  Row i (0 <= i < n, n = counts ? counts[b] : num_tokens, at most num_tokens) of
+ * (b, h) becomes token tok0[b] + i.  Every page that receives a token is quantised from what it
+ * then holds -- the tokens before tok0[b] as the values they stand for, the new ones as given:
+ * its exponent is the smallest e in [EXP_MIN, EXP_MAX] with max |finite value| <= largest * 2^e
+ * (EXP_MIN when all are 0), and code = round-to-nearest-even(value * 2^-e), saturated to the
+ * largest finite code (infinities too); NaN stays NaN.  The page's bounds cover its tokens up to the
+ * last new one (a NaN makes the bound NaN).  Rows behind the last new token keep their codes;
+ * tokens behind tok0[b] + n are no longer part of the page.  Repeating a call changes nothing.
+ * Two sequences must not append to one page in the same call.  Tokens outside the page table's
+ * row are skipped (MSKV_STATUS_DST_OOB; a negative tok0 skips the sequence), as are tokens
+ * of pages outside [0, num_pages) (MSKV_STATUS_BAD_PAGE).                                    */
+typedef struct mskv_kv8_append_desc {
+  mskv_kv8_pages pages;
+  const void* k_new;            /* element (b, h, i, d) at k_new + b*k_stride_b + h*k_stride_h */
+  const void* v_new;            /*   + i*k_stride_t (bytes) + d elements; v_new likewise      */
+  int64_t k_stride_b;
+  int64_t k_stride_h;
+  int64_t k_stride_t;
+  int64_t v_stride_b;
+  int64_t v_stride_h;
+  int64_t v_stride_t;
+  const int32_t* tok0;          /* [batch]                                            */
+  const int32_t* counts;        /* [batch]; NULL: num_tokens                          */
+  uint32_t* status;
+  int32_t dtype;                /* of k_new and v_new: MSKV_DT_BF16 / F16 / F32       */
+  int32_t num_tokens;
+} mskv_kv8_append_desc;
+int mskv_kv8_append(const mskv_kv8_append_desc* d, void* stream);
+
+/* Scores of whole pages ("blocks") from their bounds.  For block j of (b, h), j <
+ * ceil(min(lens[b], max_blocks*page_size) / page_size):
+ *   scores[(b*kv_heads + h)*scores_stride + j]
+ *     = 2^e_K * sum_d (max_d * sum_g max(q_gd, 0) + min_d * sum_g min(q_gd, 0))
+ * over the query heads g of the KV head: no token of the block has a larger GQA-summed q.k
+ * (mskv_score).  fp32; other entries are not written; a block whose page is unmapped
+ * scores -inf (MSKV_STATUS_BAD_PAGE).  q (b, hq, d) at q + b*q_stride_b + hq*q_stride_h
+ * (bytes) + d elements.                                                                     */
+typedef struct mskv_kv8_score_desc {
+  mskv_kv8_pages pages;
+  const void* q;
+  int64_t q_stride_b;
+  int64_t q_stride_h;
+  const int32_t* lens;          /* [batch] tokens                                     */
+  float* scores;
+  int64_t scores_stride;
+  uint32_t* status;
+  int32_t dtype;                /* of q: MSKV_DT_BF16 / F16                           */
+  int32_t q_heads;
+  int32_t max_blocks;           /* <= pages.max_pages, <= scores_stride               */
+  int32_t pad_;
+} mskv_kv8_score_desc;
+int mskv_kv8_block_score(const mskv_kv8_score_desc* d, void* stream);
+
+/* Attention of the last q_len (1..MSKV_KV8_MAX_QLEN) tokens of every sequence over its cache:
+ *   out[b,hq,i,:] = softmax(scale * q[b,hq,i,:] . K[b,h,t,:]) V[b,h,t,:],
+ *   t < L - q_len + 1 + i,  L = min(lens[b], max_tokens),  h = hq / (q_heads/kv_heads)
+ * (the tokens themselves already appended), over all t, or with `blocks` over the tokens of the
+ * listed pages: entry s < counts[b*kv_heads + h] of (b, h), blocks[b*blk_stride_b +
+ * h*blk_stride_h + s], is a page index within the sequence; a page listed twice counts twice.  A row
+ * that sees no token is zero.  List entries outside [0, max_pages) are skipped
+ * (MSKV_STATUS_INDEX_OOB), as are unmapped pages (MSKV_STATUS_BAD_PAGE).  Scores, softmax and
+ * sums in fp32; softmax weights enter the second product as fp16 (two fp16 terms for fp16
+ * outputs).  `workspace` must hold mskv_kv8_attention_workspace_bytes(d) bytes of device memory,
+ * 16-byte aligned; every launch writes all it reads of it.  Calls that may overlap must not share one.
+ * q (b, hq, i, d) at q + b*q_stride_b + hq*q_stride_h + i*q_stride_q (bytes) + d elements, out
+ * likewise.                                                                                 */
+typedef struct mskv_kv8_attn_desc {
+  mskv_kv8_pages pages;
+  const void* q;
+  int64_t q_stride_b;
+  int64_t q_stride_h;
+  int64_t q_stride_q;
+  void* out;
+  int64_t out_stride_b;
+  int64_t out_stride_h;
+  int64_t out_stride_q;
+  const int32_t* lens;          /* [batch] tokens                                     */
+  const int32_t* blocks;        /* NULL: the whole cache                              */
+  int64_t blk_stride_b;         /* elements                                           */
+  int64_t blk_stride_h;
+  const int32_t* counts;        /* [batch*kv_heads]; NULL: num_blocks                 */
+  void* workspace;
+  uint64_t workspace_bytes;
+  uint32_t* status;
+  float scale;
+  int32_t dtype;                /* of q and out: MSKV_DT_BF16 / F16                   */
+  int32_t q_heads;
+  int32_t q_len;
+  int32_t max_tokens;           /* bound of lens[b], <= max_pages*page_size           */
+  int32_t num_blocks;           /* width of a list                                    */
+} mskv_kv8_attn_desc;
+uint64_t mskv_kv8_attention_workspace_bytes(const mskv_kv8_attn_desc* d);
+int mskv_kv8_attention(const mskv_kv8_attn_desc* d, void* stream);
+
 /* ---- peer memory and flags (score-row exchange between the GPUs of one node) --------------
  * The shared selection's exchange of score rows (attention.py:558-572 with the KV heads on
  * several GPUs) without a collective library: device memory from mskv_ipc_alloc (zeroed;

@@ -21,6 +21,11 @@ MSKV_ERR_RANGE = 5
 # size of the device array behind mskv_sparse_attention_noalloc (MSKV_NOALLOC_ATTN_SCRATCH_BYTES)
 MSKV_NOALLOC_SCRATCH_BYTES = 8 << 20
 
+# bounds of the 8-bit cache's exponents and of a call's query positions (MSKV_KV8_*)
+KV8_EXP_MIN = -60
+KV8_EXP_MAX = 60
+KV8_MAX_QLEN = 16
+
 STATUS_INDEX_OOB = 0x1
 STATUS_BAD_PAGE = 0x2
 STATUS_DST_OOB = 0x4
@@ -108,6 +113,43 @@ class FilterDesc(C.Structure):
     ]
 
 
+class Kv8PagesDesc(C.Structure):
+    """mskv_kv8_pages: addressing of an 8-bit paged cache."""
+    _fields_ = [
+        ("k", _vp), ("v", _vp), ("exps", _vp), ("bounds", _vp), ("page_table", _vp),
+        ("stride_page", _i64), ("stride_h", _i64), ("pt_stride_b", _i64), ("num_pages", _i64),
+        ("max_pages", _i32), ("page_size", _i32), ("kv_heads", _i32), ("head_dim", _i32),
+        ("dtype", _i32), ("batch", _i32),
+    ]
+
+
+class Kv8AppendDesc(C.Structure):
+    _fields_ = [
+        ("pages", Kv8PagesDesc), ("k_new", _vp), ("v_new", _vp),
+        ("k_stride_b", _i64), ("k_stride_h", _i64), ("k_stride_t", _i64),
+        ("v_stride_b", _i64), ("v_stride_h", _i64), ("v_stride_t", _i64),
+        ("tok0", _vp), ("counts", _vp), ("status", _vp), ("dtype", _i32), ("num_tokens", _i32),
+    ]
+
+
+class Kv8ScoreDesc(C.Structure):
+    _fields_ = [
+        ("pages", Kv8PagesDesc), ("q", _vp), ("q_stride_b", _i64), ("q_stride_h", _i64),
+        ("lens", _vp), ("scores", _vp), ("scores_stride", _i64), ("status", _vp),
+        ("dtype", _i32), ("q_heads", _i32), ("max_blocks", _i32), ("pad_", _i32),
+    ]
+
+
+class Kv8AttnDesc(C.Structure):
+    _fields_ = [
+        ("pages", Kv8PagesDesc), ("q", _vp), ("q_stride_b", _i64), ("q_stride_h", _i64), ("q_stride_q", _i64),
+        ("out", _vp), ("out_stride_b", _i64), ("out_stride_h", _i64), ("out_stride_q", _i64),
+        ("lens", _vp), ("blocks", _vp), ("blk_stride_b", _i64), ("blk_stride_h", _i64), ("counts", _vp),
+        ("workspace", _vp), ("workspace_bytes", C.c_uint64), ("status", _vp), ("scale", C.c_float),
+        ("dtype", _i32), ("q_heads", _i32), ("q_len", _i32), ("max_tokens", _i32), ("num_blocks", _i32),
+    ]
+
+
 # (name, restype, argtypes) of every exported function, in header order.
 SIGNATURES = [
     ("mskv_abi_version", C.c_int, []),
@@ -129,6 +171,10 @@ SIGNATURES = [
     ("mskv_sparse_attention", C.c_int, [C.POINTER(AttnDesc), _vp]),
     ("mskv_image_filter_workspace_bytes", C.c_uint64, [_i32, _i32]),
     ("mskv_image_filter", C.c_int, [C.POINTER(FilterDesc), _vp]),
+    ("mskv_kv8_append", C.c_int, [C.POINTER(Kv8AppendDesc), _vp]),
+    ("mskv_kv8_block_score", C.c_int, [C.POINTER(Kv8ScoreDesc), _vp]),
+    ("mskv_kv8_attention_workspace_bytes", C.c_uint64, [C.POINTER(Kv8AttnDesc)]),
+    ("mskv_kv8_attention", C.c_int, [C.POINTER(Kv8AttnDesc), _vp]),
     ("mskv_ipc_handle_bytes", C.c_uint64, []),
     ("mskv_ipc_alloc", C.c_int, [C.c_uint64, C.POINTER(_vp), _vp]),
     ("mskv_ipc_open", C.c_int, [_vp, C.POINTER(_vp)]),

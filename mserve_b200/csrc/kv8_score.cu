@@ -1,0 +1,204 @@
+// Block scores of the 8-bit paged cache (mskv_kv8_block_score).
+//
+// score(block) = 2^e * sum_d (max_d * P_d + min_d * N_d), P_d = sum_g max(q_gd, 0) and
+// N_d = sum_g min(q_gd, 0) over the query heads of the KV head: the sum over the heads of each
+// head's largest possible q.k in the block, collapsed to one product of length 2D.
+//
+// Bound by the bounds' bytes (2D a block and head).  A warp takes 16 blocks at a time, straight
+// from global memory into the A fragments of mma.sync m16n8k16 (the contraction's order is free,
+// so each lane's 16 contiguous codes are four k-steps' worth).  The weights are the B operand: the fp32
+// P and N, scaled to magnitudes below 2, split in two fp16 terms in columns 0 and 1 (the second times
+// 2^12), so the products are exact and the weights keep 23 bits; lane c = 0 of a row holds
+// both columns' sums.  FMAs in fp32 would need an unpacking and an FMA per code and a
+// shuffle reduction; the tensor core needs neither.
+#include <algorithm>
+
+#include "kv8.cuh"
+
+namespace mskv {
+
+struct BlockScoreDev {
+  Kv8Dev pg;
+  const char* q;
+  int64_t q_sb, q_sh;
+  const int32_t* lens;
+  float* scores;
+  int64_t stride;
+  uint32_t* status;
+  int32_t group, max_blocks, chunks, tiles;   // chunks of a (b, h); tiles of 16 blocks a warp takes of one
+};
+
+constexpr int kBsWarps = 8;
+
+template <int D, bool E5M2, bool BF16>
+__global__ void __launch_bounds__(kBsWarps * 32) kv8_block_score_kernel(const BlockScoreDev a) {
+  constexpr int kVec = D / 32;              // 16-byte loads of a lane per block (64 codes a step of 4 lanes)
+  constexpr int kK = 2 * D / 16;            // k-steps
+  __shared__ __half s_w[2][2 * D];          // the two terms of the weights [min | max]
+  __shared__ uint32_t s_top[kBsWarps];
+
+  const int bh = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
+  const int b = bh / a.pg.heads, h = bh % a.pg.heads;
+  const int64_t len = min((int64_t)max(a.lens[b], 0), (int64_t)a.max_blocks * a.pg.page_size);
+  const int held = (int)((len + a.pg.page_size - 1) / a.pg.page_size);
+  const int first = chunk * a.tiles * kBsWarps * 16;
+  if (first >= held) return;                // the whole CTA
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  // weights: sums over the heads, then both terms at a common power of two
+  float up = 0.f, down = 0.f;
+  const int d = threadIdx.x;
+  if (d < D) {
+    const char* q = a.q + (int64_t)b * a.q_sb + (int64_t)h * a.group * a.q_sh + d * 2;
+    for (int i = 0; i < a.group; ++i) {
+      const float x = q_elem<BF16>(q + (int64_t)i * a.q_sh);
+      // a NaN reaches both sums
+      up += x < 0.f ? 0.f : x;
+      down += x > 0.f ? 0.f : x;
+    }
+  }
+  const uint32_t mu = __float_as_uint(up) & 0x7fffffffu, md = __float_as_uint(down) & 0x7fffffffu;
+  uint32_t top = max(mu < 0x7f800000u ? mu : 0u, md < 0x7f800000u ? md : 0u);
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (lane == 0) s_top[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kBsWarps; ++i) top = max(top, s_top[i]);
+  const int eq = min(max((int)(top >> 23) - 127, -120), 120);
+  if (d < D) {
+    const float f = pow2i(-eq);
+    const float w[2] = {down * f, up * f};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const __half first_term = __float2half_rn(w[i]);
+      s_w[0][i * D + d] = first_term;
+      const float rest = (w[i] - __half2float(first_term)) * 4096.f;
+      s_w[1][i * D + d] = __float2half_rn(fabsf(w[i]) <= 65504.f ? rest : 0.f);   // 0 beside an infinity or NaN
+    }
+  }
+  __syncthreads();
+  // B fragments: column g (0, 1: the two terms; others zero), k-step (v, i) = codes 64v + 16c + 4i + 0..3
+  uint32_t w0[kK], w1[kK];
+#pragma unroll
+  for (int v = 0; v < kVec; ++v)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint2 x = make_uint2(0u, 0u);
+      if (g < 2) x = *reinterpret_cast<const uint2*>(&s_w[g][64 * v + 16 * c + 4 * i]);
+      w0[v * 4 + i] = x.x;
+      w1[v * 4 + i] = x.y;
+    }
+
+  for (int t = 0; t < a.tiles; ++t) {
+    const int j0 = first + (t * kBsWarps + warp) * 16;
+    if (j0 >= held) break;
+    const int j[2] = {j0 + g, j0 + g + 8};
+    int page[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      page[r] = -2;                         // no block
+      if (j[r] < held) {
+        const int p = a.pg.page_table[(int64_t)b * a.pg.pt_stride + j[r]];
+        page[r] = p >= 0 && p < a.pg.num_pages ? p : -1;
+      }
+    }
+    uint4 x[2][kVec];
+    int e[2] = {0, 0};
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int64_t ph = (int64_t)page[r] * a.pg.heads + h;
+      if (page[r] >= 0) {
+        const uint8_t* src = a.pg.bounds + ph * 2 * D + 16 * c;
+#pragma unroll
+        for (int v = 0; v < kVec; ++v) x[r][v] = ld_stream16(src + 64 * v);
+        if (c == 0) e[r] = a.pg.exps[ph * 2];
+      } else {
+#pragma unroll
+        for (int v = 0; v < kVec; ++v) x[r][v] = make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
+    float acc[2][4] = {};                   // two chains of k-steps
+#pragma unroll
+    for (int v = 0; v < kVec; ++v) {
+      const uint32_t lo_rows[4] = {x[0][v].x, x[0][v].y, x[0][v].z, x[0][v].w};
+      const uint32_t hi_rows[4] = {x[1][v].x, x[1][v].y, x[1][v].z, x[1][v].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t a0, a1, a2, a3;
+        codes_to_half<E5M2>(lo_rows[i], a0, a2);
+        codes_to_half<E5M2>(hi_rows[i], a1, a3);
+        mma_f16(acc[i & 1], a0, a1, a2, a3, w0[v * 4 + i], w1[v * 4 + i]);
+      }
+    }
+    if (c == 0) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        if (page[r] == -2) continue;
+        float s = (acc[0][2 * r] + acc[1][2 * r]) + (acc[0][2 * r + 1] + acc[1][2 * r + 1]) * (1.f / 4096.f);
+        s = s * pow2i(e[r]) * pow2i(eq);
+        if (page[r] < 0) {
+          s = __int_as_float(0xff800000);
+          if (a.status) atomicOr(a.status, MSKV_STATUS_BAD_PAGE);
+        }
+        a.scores[(int64_t)bh * a.stride + j[r]] = s;
+      }
+    }
+  }
+}
+
+template <int D, bool E5M2>
+static int launch_block_score(const BlockScoreDev& a, bool bf16, int64_t ctas, cudaStream_t st) {
+  if (bf16) kv8_block_score_kernel<D, E5M2, true><<<(unsigned)ctas, kBsWarps * 32, 0, st>>>(a);
+  else kv8_block_score_kernel<D, E5M2, false><<<(unsigned)ctas, kBsWarps * 32, 0, st>>>(a);
+  return after_launch("mskv_kv8_block_score");
+}
+
+template <int D>
+static int block_score_cache(const BlockScoreDev& a, bool e5m2, bool bf16, int64_t ctas, cudaStream_t st) {
+  return e5m2 ? launch_block_score<D, true>(a, bf16, ctas, st) : launch_block_score<D, false>(a, bf16, ctas, st);
+}
+
+}  // namespace mskv
+
+using namespace mskv;
+
+extern "C" int mskv_kv8_block_score(const mskv_kv8_score_desc* d, void* stream) {
+  if (!d) return fail(MSKV_ERR_ARG, "mskv_kv8_block_score: NULL descriptor");
+  if (const int rc = check_kv8(d->pages, "mskv_kv8_block_score")) return rc;
+  if (d->dtype != MSKV_DT_BF16 && d->dtype != MSKV_DT_F16)
+    return fail(MSKV_ERR_DTYPE, "mskv_kv8_block_score: q must be bf16 or f16");
+  if (!d->pages.bounds) return fail(MSKV_ERR_ARG, "mskv_kv8_block_score: the cache has no bounds");
+  if (!d->q || !d->lens || !d->scores) return fail(MSKV_ERR_ARG, "mskv_kv8_block_score: NULL q, lens or scores");
+  if (d->q_heads <= 0 || d->q_heads % d->pages.kv_heads)
+    return fail(MSKV_ERR_ARG, "mskv_kv8_block_score: q_heads must be a multiple of kv_heads");
+  if (d->max_blocks < 0 || d->max_blocks > d->pages.max_pages || d->max_blocks > d->scores_stride)
+    return fail(MSKV_ERR_ARG, "mskv_kv8_block_score: max_blocks must lie in [0, min(max_pages, scores_stride)]");
+  if (((uintptr_t)d->q | (uintptr_t)d->q_stride_b | (uintptr_t)d->q_stride_h) & 1)
+    return fail(MSKV_ERR_ARG, "mskv_kv8_block_score: q must be aligned to its elements");
+  if (d->max_blocks == 0) return MSKV_OK;
+  BlockScoreDev a{};
+  a.pg = to_dev(d->pages);
+  a.q = static_cast<const char*>(d->q);
+  a.q_sb = d->q_stride_b; a.q_sh = d->q_stride_h;
+  a.lens = d->lens;
+  a.scores = d->scores;
+  a.stride = d->scores_stride;
+  a.status = d->status;
+  a.group = d->q_heads / d->pages.kv_heads;
+  a.max_blocks = d->max_blocks;
+  // Tiles a warp takes per CTA: one while that fits one wave of the GPU, up to four beyond, so the
+  // weights' set-up is shared.
+  const int64_t segs = (int64_t)a.pg.batch * a.pg.heads;
+  const int64_t rows = ((int64_t)d->max_blocks + 16 * kBsWarps - 1) / (16 * kBsWarps);
+  a.tiles = (int)std::min<int64_t>(4, std::max<int64_t>(1, segs * rows / (2 * num_sms())));
+  a.chunks = (int)((rows + a.tiles - 1) / a.tiles);
+  const int64_t ctas = segs * a.chunks;
+  if (ctas > INT_MAX) return fail(MSKV_ERR_RANGE, "mskv_kv8_block_score: too many blocks for one call");
+  const bool e5m2 = d->pages.dtype == MSKV_DT_FP8_E5M2, bf16 = d->dtype == MSKV_DT_BF16;
+  const cudaStream_t st = as_stream(stream);
+  switch (d->pages.head_dim) {
+    case 64: return block_score_cache<64>(a, e5m2, bf16, ctas, st);
+    case 128: return block_score_cache<128>(a, e5m2, bf16, ctas, st);
+    default: return block_score_cache<256>(a, e5m2, bf16, ctas, st);
+  }
+}
