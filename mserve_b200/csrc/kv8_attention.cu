@@ -55,7 +55,7 @@ struct Kv8AttnDev {
   uint32_t* status;
   float scale_log2;
   int32_t group, q_len, rows, row_tiles, segments, max_tokens, width, whole;   // whole: a CTA per segment
-  int32_t vec_q;
+  int32_t vec_q, pow2_page;
 };
 
 constexpr int kKaWarps = 8;
@@ -186,7 +186,7 @@ struct Kv8Attn {
   }
 
   struct Tile {                                   // warp-uniform
-    int page, tok, meta;                          // page < 0: nothing to read; meta: eK, eV, 16-row part of the page
+    int page, tok, exps;                          // page < 0: nothing to read; exps: eK, eV
   };
 
   // Tile `i` of (b, h) as one lane sees it.
@@ -197,7 +197,7 @@ struct Kv8Attn {
     Tile t;
     t.page = -1;
     t.tok = 0;
-    t.meta = 0;
+    t.exps = 0;
     if (a.blocks) {
       pi = a.blocks[(int64_t)b * a.blk_sb + (int64_t)h * a.blk_sh + pi];
       if (pi < 0 || pi >= a.pg.max_pages) {
@@ -212,58 +212,77 @@ struct Kv8Attn {
       if (a.status) atomicOr(a.status, MSKV_STATUS_BAD_PAGE);
       return t;
     }
-    const uint16_t e = *reinterpret_cast<const uint16_t*>(a.pg.exps + ((int64_t)page * a.pg.heads + h) * 2);
     t.page = page;
     t.tok = (int)tok;
-    t.meta = (int)e | (part << 16);
+    t.exps = *reinterpret_cast<const uint16_t*>(a.pg.exps + ((int64_t)page * a.pg.heads + h) * 2);
     return t;
   }
 
+  // Page and position of the tile that `lane` looked up (its exponents: pick_exps, once the scores are there).
   static __device__ __forceinline__ Tile pick(const Tile& mine, int lane) {
     Tile t;
     t.page = __shfl_sync(0xffffffffu, mine.page, lane);
     t.tok = __shfl_sync(0xffffffffu, mine.tok, lane);
-    t.meta = __shfl_sync(0xffffffffu, mine.meta, lane);
+    t.exps = 0;
     return t;
+  }
+
+  // Row of the page that the tile begins with.
+  static __device__ __forceinline__ int first_row(const Kv8AttnDev& a, const Tile& t) {
+    return a.pow2_page ? t.tok & (a.pg.page_size - 1) : t.tok % a.pg.page_size;
   }
 
   uint4 kr[2][kKVec];                             // K rows lane/4 and lane/4 + 8
   uint32_t vr[4][kVWords];                        // V rows 2c, 2c+1, 2c+8, 2c+9
 
+  // A tile whose 16 tokens all exist is loaded without tests; missing rows are zero.
   __device__ __forceinline__ void load_k(const Kv8AttnDev& a, const Tile& t, int h, int len, int lane) {
+    if (t.page < 0) return;
     const int g = lane >> 2, c = lane & 3;
-    const uint8_t* src = a.pg.k + (int64_t)t.page * a.pg.sp + (int64_t)h * a.pg.sh + ((t.meta >> 16) * 16 + g) * D + 16 * c;
+    const uint8_t* src = a.pg.k + (int64_t)t.page * a.pg.sp + (int64_t)h * a.pg.sh + (first_row(a, t) + g) * D + 16 * c;
+    if (t.tok + 16 <= len) {
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const bool have = t.page >= 0 && t.tok + g + 8 * r < len;
+      for (int r = 0; r < 2; ++r)
 #pragma unroll
-      for (int v = 0; v < kKVec; ++v) {
-        kr[r][v] = make_uint4(0u, 0u, 0u, 0u);
-        if (have) kr[r][v] = ld_stream16(src + 8 * r * D + 64 * v);
+        for (int v = 0; v < kKVec; ++v) kr[r][v] = ld_stream16(src + 8 * r * D + 64 * v);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int v = 0; v < kKVec; ++v) {
+          kr[r][v] = make_uint4(0u, 0u, 0u, 0u);
+          if (t.tok + g + 8 * r < len) kr[r][v] = ld_stream16(src + 8 * r * D + 64 * v);
+        }
+    }
+  }
+
+  __device__ __forceinline__ void load_v_row(int r, const uint8_t* src) {
+    if constexpr (D == 64) {
+      const uint2 x = ld_stream8(src);
+      vr[r][0] = x.x; vr[r][1] = x.y;
+    } else {
+#pragma unroll
+      for (int u = 0; u < D / 128; ++u) {
+        const uint4 x = ld_stream16(src + 128 * u);
+        vr[r][4 * u] = x.x; vr[r][4 * u + 1] = x.y; vr[r][4 * u + 2] = x.z; vr[r][4 * u + 3] = x.w;
       }
     }
   }
 
   __device__ __forceinline__ void load_v(const Kv8AttnDev& a, const Tile& t, int h, int len, int lane) {
+    if (t.page < 0) return;
     const int g = lane >> 2, c = lane & 3;
-    const uint8_t* src = a.pg.v + (int64_t)t.page * a.pg.sp + (int64_t)h * a.pg.sh + ((t.meta >> 16) * 16 + 2 * c) * D;
+    const uint8_t* src = a.pg.v + (int64_t)t.page * a.pg.sp + (int64_t)h * a.pg.sh + (first_row(a, t) + 2 * c) * D
+                         + g * (D == 64 ? 8 : 16);
+    if (t.tok + 16 <= len) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int row = (r >> 1) * 8 + (r & 1);
-      const bool have = t.page >= 0 && t.tok + 2 * c + row < len;
+      for (int r = 0; r < 4; ++r) load_v_row(r, src + ((r >> 1) * 8 + (r & 1)) * D);
+    } else {
 #pragma unroll
-      for (int i = 0; i < kVWords; ++i) vr[r][i] = 0u;
-      if (have) {
-        if constexpr (D == 64) {
-          const uint2 x = ld_stream8(src + row * D + 8 * g);
-          vr[r][0] = x.x; vr[r][1] = x.y;
-        } else {
+      for (int r = 0; r < 4; ++r) {
 #pragma unroll
-          for (int u = 0; u < D / 128; ++u) {
-            const uint4 x = ld_stream16(src + row * D + 128 * u + 16 * g);
-            vr[r][4 * u] = x.x; vr[r][4 * u + 1] = x.y; vr[r][4 * u + 2] = x.z; vr[r][4 * u + 3] = x.w;
-          }
-        }
+        for (int i = 0; i < kVWords; ++i) vr[r][i] = 0u;
+        if (t.tok + 2 * c + (r >> 1) * 8 + (r & 1) < len) load_v_row(r, src + ((r >> 1) * 8 + (r & 1)) * D);
       }
     }
   }
@@ -310,8 +329,8 @@ struct Kv8Attn {
   // Softmax weights of the tile from its raw scores: B fragments of P (and of its remainder).
   __device__ __forceinline__ void weights(const Tile& t, float (&s)[NT][4], uint32_t (&p)[NT][2], uint32_t (&rest)[NT][2],
                                           bool edge, int lane) {
-    const float tk = pow2i((int8_t)(t.meta & 0xff)), ev = (float)(int8_t)((t.meta >> 8) & 0xff);
-    const float iv = pow2i(-(int8_t)((t.meta >> 8) & 0xff));
+    const float tk = pow2i((int8_t)(t.exps & 0xff)), ev = (float)(int8_t)((t.exps >> 8) & 0xff);
+    const float iv = pow2i(-(int8_t)((t.exps >> 8) & 0xff));
     const int g = lane >> 2;
     bool over = false;
 #pragma unroll
@@ -438,15 +457,17 @@ struct Kv8Attn {
         next.page = -1;
         if (at < n) next = find(a, b, h, len, mine + at * kKaWarps);
       }
+      const int exps_of = now.exps;
       if ((i & 31) == 31) now = next;
       Tile ahead = pick(now, (i + 1) & 31);
       if (i + 1 >= n) ahead.page = -1;
       const bool edge = t.tok + 16 > seen_by_all;
       float s[NT][4];
       uint32_t p[NT][2], rest[NT][2];
-      scores(s);
+      if (t.page >= 0) scores(s);
       load_k(a, ahead, h, len, lane);
       if (t.page >= 0) {
+        t.exps = __shfl_sync(0xffffffffu, exps_of, i & 31);
         weights(t, s, p, rest, edge, lane);
         product(t, p, rest, edge, lane);
       }
@@ -531,45 +552,54 @@ struct Kv8Attn {
   }
 };
 
-// Where a CTA's part of the line of tiles begins: total tiles, the number of parts (every part has a
-// tile, and kKaWarps of them while there are that many), and the unit ((b) or, with lists,
-// (b, h)) that holds the part's first tile with the tiles before it.
-struct LineStart {
-  int64_t total, parts, before;
-  int unit;
+// The line of tiles (below 2^31) in parts of nearly equal length: the first `longer` parts have size + 1
+// tiles, the others size; every part has a tile, and kKaWarps of them while there are that many.
+struct Line {
+  uint32_t parts, size, longer;
+  uint32_t unit, before;           // the unit ((b) or, with lists, (b, h)) that holds this CTA's first tile, and the tiles before it
+
+  __device__ __forceinline__ uint32_t begin(uint32_t c) const { return c * size + min(c, longer); }
+  __device__ __forceinline__ uint32_t part_of(uint32_t x) const {
+    const uint32_t edge = longer * (size + 1);
+    return x < edge ? x / (size + 1) : longer + (x - edge) / size;
+  }
 };
 
-__device__ __forceinline__ LineStart line_start(const Kv8AttnDev& a, int64_t* scratch) {
+__device__ __forceinline__ Line line_start(const Kv8AttnDev& a, uint32_t* scratch) {
   // A unit's tiles are those of its segments: all heads and row tiles of b, or all row tiles of (b, h).
   const int units = a.blocks ? a.pg.batch * a.pg.heads : a.pg.batch;
-  const int64_t per = a.blocks ? a.row_tiles : (int64_t)a.row_tiles * a.pg.heads;
+  const uint32_t per = a.blocks ? a.row_tiles : a.row_tiles * a.pg.heads;
   const int each = (units + kKaThreads - 1) / kKaThreads;
   const int u0 = min((int)threadIdx.x * each, units), u1 = min(u0 + each, units);
-  int64_t sum = 0;
+  uint32_t sum = 0;
   for (int u = u0; u < u1; ++u)
     sum += per * (a.blocks ? kv8_tiles(a, u / a.pg.heads, u % a.pg.heads) : kv8_tiles(a, u, 0));
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int64_t upto = sum;
+  uint32_t upto = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+    const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= o) upto += x;
   }
   if (lane == 31) scratch[warp] = upto;
   __syncthreads();
-  int64_t total = 0, base = 0;
+  uint32_t total = 0, base = 0;
 #pragma unroll
   for (int w = 0; w < kKaWarps; ++w) {
     if (w < warp) base += scratch[w];
     total += scratch[w];
   }
-  const int64_t parts = min((int64_t)gridDim.x, (total + kKaWarps - 1) / kKaWarps);
-  const int64_t begin = parts ? total * blockIdx.x / parts : 0;
-  int64_t before = base + upto - sum;
-  if (sum > 0 && begin >= before && begin < before + sum) {
+  Line line{};
+  line.parts = min(gridDim.x, (total + kKaWarps - 1) / kKaWarps);
+  if (line.parts == 0) return line;
+  line.size = total / line.parts;
+  line.longer = total - line.size * line.parts;
+  const uint32_t begin = line.begin(blockIdx.x);
+  uint32_t before = base + upto - sum;
+  if (begin >= before && begin - before < sum) {
     for (int u = u0; u < u1; ++u) {
-      const int64_t n = per * (a.blocks ? kv8_tiles(a, u / a.pg.heads, u % a.pg.heads) : kv8_tiles(a, u, 0));
-      if (begin < before + n) {
+      const uint32_t n = per * (a.blocks ? kv8_tiles(a, u / a.pg.heads, u % a.pg.heads) : kv8_tiles(a, u, 0));
+      if (begin - before < n) {
         scratch[kKaWarps] = u;
         scratch[kKaWarps + 1] = before;
         break;
@@ -578,7 +608,9 @@ __device__ __forceinline__ LineStart line_start(const Kv8AttnDev& a, int64_t* sc
     }
   }
   __syncthreads();
-  return {total, parts, scratch[kKaWarps + 1], (int)scratch[kKaWarps]};
+  line.unit = scratch[kKaWarps];
+  line.before = scratch[kKaWarps + 1];
+  return line;
 }
 
 template <int D, int NT, bool E5M2, bool BF16>
@@ -586,7 +618,7 @@ __global__ void __launch_bounds__(kKaThreads, D <= 128 && NT == 1 ? 2 : 1) kv8_a
   using K = Kv8Attn<D, NT, E5M2, BF16>;
   extern __shared__ __align__(16) char smem_raw[];
   typename K::Smem& sm = *reinterpret_cast<typename K::Smem*>(smem_raw);
-  __shared__ int64_t s_line[kKaWarps + 2];
+  __shared__ uint32_t s_line[kKaWarps + 2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   K k;
   if (a.whole) {
@@ -598,14 +630,14 @@ __global__ void __launch_bounds__(kKaThreads, D <= 128 && NT == 1 ? 2 : 1) kv8_a
     k.finish(a, sm, b, h, rt, -1, warp, lane);
     return;
   }
-  const LineStart line = line_start(a, s_line);
+  const Line line = line_start(a, s_line);
   if (blockIdx.x < line.parts) {
-    const int64_t begin = line.total * blockIdx.x / line.parts, end = line.total * (blockIdx.x + 1) / line.parts;
+    const uint32_t begin = line.begin(blockIdx.x), end = line.begin(blockIdx.x + 1);
     // segment of `begin`
     int b, h, rt;
-    int n = a.blocks ? kv8_tiles(a, line.unit / a.pg.heads, line.unit % a.pg.heads) : kv8_tiles(a, line.unit, 0);
-    int64_t seg = (begin - line.before) / n;
-    int64_t start = line.before + seg * n;            // the segment's first tile on the line
+    uint32_t n = a.blocks ? kv8_tiles(a, line.unit / a.pg.heads, line.unit % a.pg.heads) : kv8_tiles(a, line.unit, 0);
+    const uint32_t seg = (begin - line.before) / n;
+    uint32_t start = line.before + seg * n;           // the segment's first tile on the line
     rt = (int)(seg % a.row_tiles);
     if (a.blocks) {
       b = line.unit / a.pg.heads;
@@ -614,19 +646,17 @@ __global__ void __launch_bounds__(kKaThreads, D <= 128 && NT == 1 ? 2 : 1) kv8_a
       b = line.unit;
       h = (int)(seg / a.row_tiles);
     }
-    int64_t at = begin;
+    uint32_t at = begin;
     for (;;) {
-      const int first = (int)(at - start), last = (int)min((int64_t)n, end - start);
+      const uint32_t first = at - start, last = min(n, end - start);
       const bool cut = first > 0 || last < n;
       const int len = kv8_len(a, b);
       k.load_q(a, b, h, rt, len, lane);
       k.stream(a, b, h, len, first, last, warp, lane);
       k.finish(a, sm, b, h, rt, cut ? 2 * (int)blockIdx.x + (at == begin ? 0 : 1) : -1, warp, lane);
-      if (first == 0 && threadIdx.x == 0) {
-        // part of tile x: the last c with total*c/parts <= x
-        const int64_t hi = ((start + n) * line.parts - 1) / line.total;
-        a.info[((int64_t)b * a.pg.heads + h) * a.row_tiles + rt] = make_int4((int)blockIdx.x, (int)hi, at == begin ? 0 : 1, 0);
-      }
+      if (first == 0 && threadIdx.x == 0)
+        a.info[((int64_t)b * a.pg.heads + h) * a.row_tiles + rt] =
+            make_int4((int)blockIdx.x, (int)line.part_of(start + n - 1), at == begin ? 0 : 1, 0);
       at = start + last;
       if (at >= end) break;
       start += n;
@@ -775,6 +805,9 @@ static int check_attn(const mskv_kv8_attn_desc* d) {
   const int64_t row_tiles = ((int64_t)d->q_heads / d->pages.kv_heads * d->q_len + 7) / 8;
   if (row_tiles * d->pages.batch * d->pages.kv_heads > INT_MAX / 16)
     return fail(MSKV_ERR_RANGE, "%s: too many query rows for one call", what);
+  const int64_t most = d->blocks ? (int64_t)d->num_blocks * (d->pages.page_size / 16) : ((int64_t)d->max_tokens + 15) / 16;
+  if (row_tiles * d->pages.batch * d->pages.kv_heads * most > INT_MAX / 2)
+    return fail(MSKV_ERR_RANGE, "%s: too many tokens for one call", what);
   if (!(fabsf(d->scale) <= 3e38f)) return fail(MSKV_ERR_ARG, "%s: scale must be finite", what);
   return MSKV_OK;
 }
@@ -824,6 +857,7 @@ extern "C" int mskv_kv8_attention(const mskv_kv8_attn_desc* d, void* stream) {
   a.width = d->num_blocks;
   a.whole = p.whole;
   a.vec_q = (q_bits & 15) == 0;
+  a.pow2_page = (a.pg.page_size & (a.pg.page_size - 1)) == 0;
   const bool e5m2 = d->pages.dtype == MSKV_DT_FP8_E5M2, bf16 = d->dtype == MSKV_DT_BF16;
   const cudaStream_t st = as_stream(stream);
   switch (d->pages.head_dim) {
