@@ -19,23 +19,27 @@
 //
 // Bound by the codes' bytes (2D a token and KV head).  mma.sync m16n8k16 with the tokens on M:
 // S^T = K Q^T, O^T = V^T P^T, so the 8 columns hold the query rows (16 rows: two column tiles).
-// A warp owns a tile: 16-byte loads straight from global memory into the fragments' registers -- the
-// contraction's order is free, so a lane's 16 contiguous codes of a K row are four k-steps', and
-// those of four V rows are eight row tiles' (byte permutations pair the tokens) -- no shared memory and
-// no barrier on the way; K of the next tile is in flight during the softmax, V during the next product.
+// A warp owns a tile.  The contraction's order is free, so a lane's 16 contiguous codes of a K row are four
+// k-steps', and those of four V rows are eight row tiles' (byte permutations pair the tokens): 16-byte loads
+// straight from global memory into the fragments' registers, no shared memory and no barrier on the way; K of
+// the next tile is in flight during the softmax, V during the next scores.  (The same chunks through
+// cp.async into a ring of three tiles a warp: 257 us instead of 185 for 16 x 32768 tokens of 8 heads.)
 // A tcgen05 MMA would need 64 or 128 rows of f16 operands staged in shared memory after a
 // conversion there; the legacy pipe is a fifth busy at the memory's speed.
 //
-// Split: all tiles of all (sequence, KV head, row tile) segments form one line, cut into equal parts
-// for the CTAs however ragged the lengths are (a scan over the lengths in every CTA).  The 8 warps of a
-// CTA take a segment's tiles in turn and merge in shared memory; a segment cut by a CTA border goes
-// through the workspace and a second kernel.  Segments of few tiles go to one CTA each
-// and need neither.
+// Split: all tiles of all (sequence, KV head, row tile) segments form one line, cut into parts
+// for the CTAs however ragged the lengths are (a scan over the lengths in every warp).  The 8 warps of a
+// CTA take a segment's tiles in turn and merge in shared memory; a segment of several CTAs goes
+// through the workspace and a second kernel.  Segments of few tiles go to one CTA or cluster
+// each and need neither.
+#include <cooperative_groups.h>
 #include <math.h>
 
 #include <algorithm>
 
 #include "kv8.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace mskv {
 
@@ -54,8 +58,8 @@ struct Kv8AttnDev {
   float* part_o;                   // [2 * CTAs][rows][D]
   uint32_t* status;
   float scale_log2;
-  int32_t group, q_len, rows, row_tiles, segments, max_tokens, width, whole;   // whole: a CTA per segment
-  int32_t vec_q, pow2_page;
+  int32_t group, q_len, rows, row_tiles, segments, max_tokens, width, cluster;   // cluster: CTAs that share a segment, 0: the line
+  int32_t vec_q, pow2_page, aligned;
 };
 
 constexpr int kKaWarps = 8;
@@ -89,6 +93,35 @@ __device__ __forceinline__ uint32_t nonfinite_bytes(uint32_t w) {
   return E5M2 ? __vcmpgtu4(w & 0x7f7f7f7fu, 0x7b7b7b7bu) : __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu);
 }
 
+// The line of tiles (below 2^31) of all segments, cut into parts, one for each CTA.
+// Few segments with few tiles (a.aligned): parts do not cross segments.  A segment of n
+// tiles has ceil(n / size) parts of nearly equal length; size = ceil(total / (CTAs - segments))
+// makes them at most as many as the CTAs.  A CTA that starts a second segment starts its pipeline
+// and merges again, about 4 us, which is worth more than the even shares when there are few tiles.
+// Otherwise `parts` parts of nearly equal length, the first `longer` of size + 1 tiles, the others of size.
+// Every part has a tile.
+struct Line {
+  uint32_t parts, size, longer;
+  uint32_t begin, end;             // this CTA's tiles
+  uint32_t unit, before;           // the unit ((b) or, with lists, (b, h)) of its first tile, and the tiles before the unit
+
+  __device__ __forceinline__ uint32_t even_begin(uint32_t c) const { return c * size + min(c, longer); }
+  // Last part of the segment of tiles [start, start + n) whose first part is c.
+  __device__ __forceinline__ uint32_t last_part(bool aligned, uint32_t c, uint32_t start, uint32_t n) const {
+    if (aligned) return c + (n + size - 1) / size - 1;
+    const uint32_t x = start + n - 1, edge = longer * (size + 1);
+    return x < edge ? x / (size + 1) : longer + (x - edge) / size;
+  }
+};
+
+// A CTA's place: the segment, its tiles and its first one's place on the line, the CTA's tiles [at, end)
+// from this segment on, its first of all.
+struct Place {
+  int b, h, rt;
+  uint32_t n, start, at, end, begin;
+  Line line;
+};
+
 template <int D, int NT, bool E5M2, bool BF16>
 struct Kv8Attn {
   static constexpr int kRows = NT * 8;
@@ -99,82 +132,87 @@ struct Kv8Attn {
   static constexpr bool kTwoTerms = !BF16;        // P as two fp16 terms
 
   struct Smem {
+    float o[kKaWarps][kRows][kOStride];           // the warps' sums; o[0], m[0] and l[0] then the CTA's
     float m[kKaWarps][kRows], l[kKaWarps][kRows];
-    float o[kKaWarps][kRows][kOStride];
+    __half q[kRows][D + 8];
+    float f[kRows];
+    int lim[kRows];                               // tokens that a row sees
   };
 
   uint32_t qf[NT][kKVec * 4][2];
   float f[NT][2];                                 // scale * log2(e) * 2^(row exponent) of the lane's two columns
   float m[NT][2], l[NT][2];
   float o[NT][kOT][4];
-  int lim[NT][2];                                 // tokens that the two columns see
 
-  // Query rows of the segment as B fragments; column n = lane/4 of column tile nt is row
-  // 8*(row tile*NT + nt) + n = position * group + head.
-  __device__ __forceinline__ void load_q(const Kv8AttnDev& a, int b, int h, int rt, int len, int lane) {
-    const int g = lane >> 2, c = lane & 3;
+  // Query rows of the segment to shared memory: a warp takes a row (NT of them), a lane D/32 neighbouring
+  // elements, scaled to a largest magnitude in [1, 2).  Row 8*(row tile*NT + nt) + n is position * group + head.
+  static __device__ __forceinline__ void stage_q(const Kv8AttnDev& a, Smem& sm, int b, int h, int rt, int len, int warp, int lane) {
+    constexpr int kPer = D / 32;
+#pragma unroll 1
+    for (int n = warp; n < kRows; n += kKaWarps) {
+      const int r = rt * kRows + n;
+      float x[kPer];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int r = (rt * NT + nt) * 8 + g;
-      float x[kKVec][16];
+      for (int i = 0; i < kPer; ++i) x[i] = 0.f;
       if (r < a.rows) {
-        const int pos = r / a.group, head = h * a.group + r % a.group;
-        const char* src = a.q + (int64_t)b * a.q_sb + (int64_t)head * a.q_sh + (int64_t)pos * a.q_sq + 32 * c;
-#pragma unroll
-        for (int v = 0; v < kKVec; ++v) {
-          uint32_t w[8];
-          if (a.vec_q) {
-            const uint4 p0 = *reinterpret_cast<const uint4*>(src + 128 * v);
-            const uint4 p1 = *reinterpret_cast<const uint4*>(src + 128 * v + 16);
-            w[0] = p0.x; w[1] = p0.y; w[2] = p0.z; w[3] = p0.w; w[4] = p1.x; w[5] = p1.y; w[6] = p1.z; w[7] = p1.w;
+        const int pos = r / a.group, head = h * a.group + r - pos * a.group;
+        const char* src = a.q + (int64_t)b * a.q_sb + (int64_t)head * a.q_sh + (int64_t)pos * a.q_sq + lane * (kPer * 2);
+        if (a.vec_q) {
+          uint32_t w[kPer / 2];
+          if constexpr (kPer == 2) {
+            w[0] = *reinterpret_cast<const uint32_t*>(src);
+          } else if constexpr (kPer == 4) {
+            const uint2 y = *reinterpret_cast<const uint2*>(src);
+            w[0] = y.x; w[1] = y.y;
           } else {
-            const uint16_t* s = reinterpret_cast<const uint16_t*>(src + 128 * v);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = (uint32_t)s[2 * i] | ((uint32_t)s[2 * i + 1] << 16);
+            const uint4 y = *reinterpret_cast<const uint4*>(src);
+            w[0] = y.x; w[1] = y.y; w[2] = y.z; w[3] = y.w;
           }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if constexpr (BF16) {
-              x[v][2 * i] = __uint_as_float(w[i] << 16);
-              x[v][2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-            } else {
-              const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-              x[v][2 * i] = y.x;
-              x[v][2 * i + 1] = y.y;
-            }
+          for (int i = 0; i < kPer; ++i) {
+            const uint16_t u = (uint16_t)(i & 1 ? w[i / 2] >> 16 : w[i / 2]);
+            x[i] = BF16 ? __uint_as_float((uint32_t)u << 16) : __half2float(__ushort_as_half(u));
           }
+        } else {
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) x[i] = q_elem<BF16>(src + 2 * i);
         }
-      } else {
-#pragma unroll
-        for (int v = 0; v < kKVec; ++v)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) x[v][i] = 0.f;
       }
       uint32_t top = 0;
 #pragma unroll
-      for (int v = 0; v < kKVec; ++v)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const uint32_t u = __float_as_uint(x[v][i]) & 0x7fffffffu;
-          top = max(top, u < 0x7f800000u ? u : 0u);
-        }
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      for (int i = 0; i < kPer; ++i) {
+        const uint32_t u = __float_as_uint(x[i]) & 0x7fffffffu;
+        top = max(top, u < 0x7f800000u ? u : 0u);
+      }
+      top = __reduce_max_sync(0xffffffffu, top);
       const int e = top ? min(max((int)(top >> 23) - 127, -120), 120) : 0;
       const float inv = pow2i(-e);
 #pragma unroll
-      for (int v = 0; v < kKVec; ++v)
+      for (int i = 0; i < kPer; i += 2)
+        *reinterpret_cast<uint32_t*>(&sm.q[n][lane * kPer + i]) = pack_half2(x[i] * inv, x[i + 1] * inv);
+      if (lane == 0) {
+        sm.f[n] = a.scale_log2 * pow2i(e);
+        sm.lim[n] = len - a.q_len + 1 + (r < a.rows ? r / a.group : a.q_len - 1);
+      }
+    }
+  }
+
+  // The staged rows as B fragments: column n = lane/4 of column tile nt is row 8*nt + n, the lane's k-steps
+  // of a 64-element stretch are its 16 contiguous elements.  Resets the running sums.
+  __device__ __forceinline__ void start(const Smem& sm, int lane) {
+    const int g = lane >> 2, c = lane & 3;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          qf[nt][v * 4 + i][0] = pack_half2(x[v][4 * i] * inv, x[v][4 * i + 1] * inv);
-          qf[nt][v * 4 + i][1] = pack_half2(x[v][4 * i + 2] * inv, x[v][4 * i + 3] * inv);
-        }
-      const float row_f = a.scale_log2 * pow2i(e);
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int v = 0; v < kKVec; ++v) {
+        const uint4* src = reinterpret_cast<const uint4*>(&sm.q[nt * 8 + g][64 * v + 16 * c]);
+        const uint4 x = src[0], y = src[1];
+        qf[nt][v * 4][0] = x.x; qf[nt][v * 4][1] = x.y; qf[nt][v * 4 + 1][0] = x.z; qf[nt][v * 4 + 1][1] = x.w;
+        qf[nt][v * 4 + 2][0] = y.x; qf[nt][v * 4 + 2][1] = y.y; qf[nt][v * 4 + 3][0] = y.z; qf[nt][v * 4 + 3][1] = y.w;
+      }
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        f[nt][k] = __shfl_sync(0xffffffffu, row_f, (2 * c + k) * 4);
-        const int rc = (rt * NT + nt) * 8 + 2 * c + k;
-        lim[nt][k] = len - a.q_len + 1 + (rc < a.rows ? rc / a.group : a.q_len - 1);
+        f[nt][k] = sm.f[nt * 8 + 2 * c + k];
         m[nt][k] = kNoMax;
         l[nt][k] = 0.f;
       }
@@ -185,8 +223,8 @@ struct Kv8Attn {
     }
   }
 
-  struct Tile {                                   // warp-uniform
-    int page, tok, exps;                          // page < 0: nothing to read; exps: eK, eV
+  struct Tile {                                   // one lane's lookup
+    int page, tok, exps;                          // page < 0: nothing to read; exps: eK, eV, bit 16: there are tokens
   };
 
   // Tile `i` of (b, h) as one lane sees it.
@@ -214,33 +252,25 @@ struct Kv8Attn {
     }
     t.page = page;
     t.tok = (int)tok;
-    t.exps = *reinterpret_cast<const uint16_t*>(a.pg.exps + ((int64_t)page * a.pg.heads + h) * 2);
+    t.exps = *reinterpret_cast<const uint16_t*>(a.pg.exps + ((int64_t)page * a.pg.heads + h) * 2) | 0x10000;
     return t;
-  }
-
-  // Page and position of the tile that `lane` looked up (its exponents: pick_exps, once the scores are there).
-  static __device__ __forceinline__ Tile pick(const Tile& mine, int lane) {
-    Tile t;
-    t.page = __shfl_sync(0xffffffffu, mine.page, lane);
-    t.tok = __shfl_sync(0xffffffffu, mine.tok, lane);
-    t.exps = 0;
-    return t;
-  }
-
-  // Row of the page that the tile begins with.
-  static __device__ __forceinline__ int first_row(const Kv8AttnDev& a, const Tile& t) {
-    return a.pow2_page ? t.tok & (a.pg.page_size - 1) : t.tok % a.pg.page_size;
   }
 
   uint4 kr[2][kKVec];                             // K rows lane/4 and lane/4 + 8
   uint32_t vr[4][kVWords];                        // V rows 2c, 2c+1, 2c+8, 2c+9
 
+  // Row of the page that a tile begins with.
+  static __device__ __forceinline__ int64_t tile_offset(const Kv8AttnDev& a, int page, int tok, int h) {
+    const int row = a.pow2_page ? tok & (a.pg.page_size - 1) : tok % a.pg.page_size;
+    return (int64_t)page * a.pg.sp + (int64_t)h * a.pg.sh + row * D;
+  }
+
   // A tile whose 16 tokens all exist is loaded without tests; missing rows are zero.
-  __device__ __forceinline__ void load_k(const Kv8AttnDev& a, const Tile& t, int h, int len, int lane) {
-    if (t.page < 0) return;
+  __device__ __forceinline__ void load_k(const Kv8AttnDev& a, int page, int tok, int h, int len, int lane) {
+    if (page < 0) return;
     const int g = lane >> 2, c = lane & 3;
-    const uint8_t* src = a.pg.k + (int64_t)t.page * a.pg.sp + (int64_t)h * a.pg.sh + (first_row(a, t) + g) * D + 16 * c;
-    if (t.tok + 16 <= len) {
+    const uint8_t* src = a.pg.k + tile_offset(a, page, tok, h) + g * D + 16 * c;
+    if (tok + 16 <= len) {
 #pragma unroll
       for (int r = 0; r < 2; ++r)
 #pragma unroll
@@ -251,7 +281,7 @@ struct Kv8Attn {
 #pragma unroll
         for (int v = 0; v < kKVec; ++v) {
           kr[r][v] = make_uint4(0u, 0u, 0u, 0u);
-          if (t.tok + g + 8 * r < len) kr[r][v] = ld_stream16(src + 8 * r * D + 64 * v);
+          if (tok + g + 8 * r < len) kr[r][v] = ld_stream16(src + 8 * r * D + 64 * v);
         }
     }
   }
@@ -269,12 +299,11 @@ struct Kv8Attn {
     }
   }
 
-  __device__ __forceinline__ void load_v(const Kv8AttnDev& a, const Tile& t, int h, int len, int lane) {
-    if (t.page < 0) return;
+  __device__ __forceinline__ void load_v(const Kv8AttnDev& a, int page, int tok, int h, int len, int lane) {
+    if (page < 0) return;
     const int g = lane >> 2, c = lane & 3;
-    const uint8_t* src = a.pg.v + (int64_t)t.page * a.pg.sp + (int64_t)h * a.pg.sh + (first_row(a, t) + 2 * c) * D
-                         + g * (D == 64 ? 8 : 16);
-    if (t.tok + 16 <= len) {
+    const uint8_t* src = a.pg.v + tile_offset(a, page, tok, h) + 2 * c * D + g * (D == 64 ? 8 : 16);
+    if (tok + 16 <= len) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) load_v_row(r, src + ((r >> 1) * 8 + (r & 1)) * D);
     } else {
@@ -282,7 +311,7 @@ struct Kv8Attn {
       for (int r = 0; r < 4; ++r) {
 #pragma unroll
         for (int i = 0; i < kVWords; ++i) vr[r][i] = 0u;
-        if (t.tok + 2 * c + (r >> 1) * 8 + (r & 1) < len) load_v_row(r, src + ((r >> 1) * 8 + (r & 1)) * D);
+        if (tok + 2 * c + (r >> 1) * 8 + (r & 1) < len) load_v_row(r, src + ((r >> 1) * 8 + (r & 1)) * D);
       }
     }
   }
@@ -327,10 +356,10 @@ struct Kv8Attn {
   }
 
   // Softmax weights of the tile from its raw scores: B fragments of P (and of its remainder).
-  __device__ __forceinline__ void weights(const Tile& t, float (&s)[NT][4], uint32_t (&p)[NT][2], uint32_t (&rest)[NT][2],
+  __device__ __forceinline__ void weights(const Smem& sm, int tok, int exps, float (&s)[NT][4], uint32_t (&p)[NT][2], uint32_t (&rest)[NT][2],
                                           bool edge, int lane) {
-    const float tk = pow2i((int8_t)(t.exps & 0xff)), ev = (float)(int8_t)((t.exps >> 8) & 0xff);
-    const float iv = pow2i(-(int8_t)((t.exps >> 8) & 0xff));
+    const float tk = pow2i((int8_t)(exps & 0xff)), ev = (float)(int8_t)((exps >> 8) & 0xff);
+    const float iv = pow2i(-(int8_t)((exps >> 8) & 0xff));
     const int g = lane >> 2;
     bool over = false;
 #pragma unroll
@@ -341,7 +370,7 @@ struct Kv8Attn {
       if (edge) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          if (t.tok + g + (k >> 1) * 8 >= lim[nt][k & 1]) s[nt][k] = -INFINITY;
+          if (tok + g + (k >> 1) * 8 >= sm.lim[nt * 8 + 2 * (lane & 3) + (k & 1)]) s[nt][k] = -INFINITY;
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) over |= s[nt][k] > m[nt][k & 1] + 8.f;
@@ -386,9 +415,9 @@ struct Kv8Attn {
   }
 
   // O^T += V^T P^T of the tile in vr; vr is free afterwards.
-  __device__ __forceinline__ void product(const Tile& t, const uint32_t (&p)[NT][2], const uint32_t (&rest)[NT][2],
+  __device__ __forceinline__ void product(const Smem& sm, int tok, const uint32_t (&p)[NT][2], const uint32_t (&rest)[NT][2],
                                           bool edge, int lane) {
-    if (edge) not_finite(t, lane);
+    if (edge) not_finite(sm, tok, lane);
 #pragma unroll
     for (int i = 0; i < kVWords; ++i) {
       const uint32_t w[4] = {vr[0][i], vr[1][i], vr[2][i], vr[3][i]};
@@ -404,7 +433,7 @@ struct Kv8Attn {
   // that see it and no other, but 0 * NaN is NaN.  Such codes are counted per row in a product of
   // their own (1 for each, times 1 for each row that sees the token), turn the row's sums to NaN
   // and are cleared.
-  __device__ __forceinline__ void not_finite(const Tile& t, int lane) {
+  __device__ __forceinline__ void not_finite(const Smem& sm, int tok, int lane) {
     bool any = false;
 #pragma unroll
     for (int r = 0; r < 4; ++r)
@@ -418,7 +447,8 @@ struct Kv8Attn {
       uint32_t sees[2];
 #pragma unroll
       for (int k = 0; k < 2; ++k)
-        sees[k] = transpose8x8(pack_half2(t.tok + g + 8 * k < lim[nt][0] ? 1.f : 0.f, t.tok + g + 8 * k < lim[nt][1] ? 1.f : 0.f));
+        sees[k] = transpose8x8(pack_half2(tok + g + 8 * k < sm.lim[nt * 8 + 2 * (lane & 3)] ? 1.f : 0.f,
+                                          tok + g + 8 * k < sm.lim[nt * 8 + 2 * (lane & 3) + 1] ? 1.f : 0.f));
 #pragma unroll
       for (int i = 0; i < kVWords; ++i) {
         float n0[4] = {}, n1[4] = {};
@@ -439,45 +469,54 @@ struct Kv8Attn {
       for (int i = 0; i < kVWords; ++i) vr[r][i] &= ~nonfinite_bytes<E5M2>(vr[r][i]);
   }
 
-  // This warp's share (every kKaWarps-th) of tiles [first, last) of (b, h).
-  __device__ __forceinline__ void stream(const Kv8AttnDev& a, int b, int h, int len, int first, int last, int warp, int lane) {
+  // The CTA's tiles of the segment: the warp's share (every kKaWarps-th).  The first tile's codes are on their way
+  // while the query is staged.
+  __device__ __forceinline__ void piece(const Kv8AttnDev& a, Smem& sm, const Place& at, int warp, int lane) {
+    const int b = at.b, h = at.h, rt = at.rt;
+    const int first = (int)(at.at - at.start), last = (int)min(at.n, at.end - at.start);
+    const int len = kv8_len(a, b);
     const int seen_by_all = len - a.q_len + 1;    // tokens below: every row sees them
     const int mine = first + warp;
-    if (mine >= last) return;
-    const int n = (last - mine + kKaWarps - 1) / kKaWarps;
+    const int n = mine < last ? (last - mine + kKaWarps - 1) / kKaWarps : 0;
     // lane j describes this warp's tile 32*k + j; the next 32 are looked up halfway through
     Tile now{-1, 0, 0}, next{-1, 0, 0};
     if (lane < n) now = find(a, b, h, len, mine + lane * kKaWarps);
-    Tile t = pick(now, 0);
-    load_k(a, t, h, len, lane);
-    load_v(a, t, h, len, lane);
+    int page = __shfl_sync(0xffffffffu, now.page, 0), tok = __shfl_sync(0xffffffffu, now.tok, 0);
+    load_k(a, page, tok, h, len, lane);
+    load_v(a, page, tok, h, len, lane);
+    stage_q(a, sm, b, h, rt, len, warp, lane);
+    __syncthreads();
+    start(sm, lane);
+#pragma unroll 1
     for (int i = 0; i < n; ++i) {
       if ((i & 31) == 16) {
-        const int at = (i & ~31) + 32 + lane;
-        next.page = -1;
-        if (at < n) next = find(a, b, h, len, mine + at * kKaWarps);
+        const int j = (i & ~31) + 32 + lane;
+        next = Tile{-1, 0, 0};
+        if (j < n) next = find(a, at.b, h, len, (int)(at.at - at.start) + warp + j * kKaWarps);
       }
-      const int exps_of = now.exps;
+      const int exps = __shfl_sync(0xffffffffu, now.exps, i & 31);
       if ((i & 31) == 31) now = next;
-      Tile ahead = pick(now, (i + 1) & 31);
-      if (i + 1 >= n) ahead.page = -1;
-      const bool edge = t.tok + 16 > seen_by_all;
+      int page_ahead = __shfl_sync(0xffffffffu, now.page, (i + 1) & 31);
+      const int tok_ahead = __shfl_sync(0xffffffffu, now.tok, (i + 1) & 31);
+      if (i + 1 >= n) page_ahead = -1;
+      const bool edge = tok + 16 > seen_by_all;
       float s[NT][4];
       uint32_t p[NT][2], rest[NT][2];
-      if (t.page >= 0) scores(s);
-      load_k(a, ahead, h, len, lane);
-      if (t.page >= 0) {
-        t.exps = __shfl_sync(0xffffffffu, exps_of, i & 31);
-        weights(t, s, p, rest, edge, lane);
-        product(t, p, rest, edge, lane);
+      if (page >= 0) scores(s);
+      load_k(a, page_ahead, tok_ahead, h, len, lane);
+      if (page >= 0) {
+        weights(sm, tok, exps, s, p, rest, edge, lane);
+        product(sm, tok, p, rest, edge, lane);
       }
-      load_v(a, ahead, h, len, lane);
-      t = ahead;
+      load_v(a, page_ahead, tok_ahead, h, len, lane);
+      page = page_ahead;
+      tok = tok_ahead;
     }
+    collect(sm, warp, lane);
   }
 
-  // Merges the warps and writes the segment's rows: to `out`, or (slot >= 0) to the workspace.
-  __device__ __forceinline__ void finish(const Kv8AttnDev& a, Smem& sm, int b, int h, int rt, int slot, int warp, int lane) {
+  // The warps' (m, l, O) to shared memory, O relative to the CTA's m.
+  __device__ __forceinline__ void collect(Smem& sm, int warp, int lane) {
     const int g = lane >> 2, c = lane & 3;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -512,26 +551,84 @@ struct Kv8Attn {
         }
       }
     __syncthreads();
+  }
+
+  // Sums of the CTA for dims d .. d+3 of row r, after collect.
+  struct Part {
+    float4 x;
+    float top, sum;
+  };
+  static __device__ __forceinline__ Part cta_part(const Smem& sm, int r, int d) {
+    Part y{make_float4(0.f, 0.f, 0.f, 0.f), sm.m[0][r], 0.f};
+#pragma unroll
+    for (int w = 1; w < kKaWarps; ++w) y.top = fmaxf(y.top, sm.m[w][r]);
+#pragma unroll
+    for (int w = 0; w < kKaWarps; ++w) {
+      const float4 z = *reinterpret_cast<const float4*>(&sm.o[w][r][d]);
+      y.x.x += z.x; y.x.y += z.y; y.x.z += z.z; y.x.w += z.w;
+      y.sum += sm.l[w][r] * exp2_fast(sm.m[w][r] - y.top);
+    }
+    return y;
+  }
+
+  // Writes the CTA's rows after a piece: to `out`, or (slot >= 0) to the workspace.
+  static __device__ __forceinline__ void finish(const Kv8AttnDev& a, const Smem& sm, const Place& at, int slot) {
+#pragma unroll 1
     for (int i = threadIdx.x; i < kRows * D / 4; i += kKaThreads) {
       const int r = i / (D / 4), d = (i % (D / 4)) * 4;
-      float top = sm.m[0][r], sum = 0.f;
-#pragma unroll
-      for (int w = 1; w < kKaWarps; ++w) top = fmaxf(top, sm.m[w][r]);
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < kKaWarps; ++w) {
-        const float4 y = *reinterpret_cast<const float4*>(&sm.o[w][r][d]);
-        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
-        sum += sm.l[w][r] * exp2_fast(sm.m[w][r] - top);
-      }
+      const Part y = cta_part(sm, r, d);
       if (slot >= 0) {
-        *reinterpret_cast<float4*>(a.part_o + ((int64_t)slot * kRows + r) * D + d) = x;
-        if (d == 0) *reinterpret_cast<float2*>(a.part_ml + ((int64_t)slot * kRows + r) * 2) = make_float2(top, sum);
-      } else if (rt * kRows + r < a.rows) {
-        write_out(a, b, h, rt * kRows + r, d, x, sum);
+        *reinterpret_cast<float4*>(a.part_o + ((int64_t)slot * kRows + r) * D + d) = y.x;
+        if (d == 0) *reinterpret_cast<float2*>(a.part_ml + ((int64_t)slot * kRows + r) * 2) = make_float2(y.top, y.sum);
+      } else if (at.rt * kRows + r < a.rows) {
+        write_out(a, at.b, at.h, at.rt * kRows + r, d, y.x, y.sum);
       }
     }
-    __syncthreads();                              // the next segment reuses the buffers
+  }
+
+  // The same for a cluster of `ctas` CTAs that share a segment: every CTA sums its warps in place, then finishes the
+  // rows of its rank from all the CTAs' shared memory.
+  static __device__ __forceinline__ void finish_cluster(const Kv8AttnDev& a, Smem& sm, const Place& at, int rank, int ctas) {
+    constexpr int kEach = kRows * D / 4 / kKaThreads > 0 ? kRows * D / 4 / kKaThreads : 1;
+    Part y[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int i = threadIdx.x + e * kKaThreads;
+      if (i < kRows * D / 4) y[e] = cta_part(sm, i / (D / 4), (i % (D / 4)) * 4);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int i = threadIdx.x + e * kKaThreads, r = i / (D / 4), d = (i % (D / 4)) * 4;
+      if (i < kRows * D / 4) {
+        *reinterpret_cast<float4*>(&sm.o[0][r][d]) = y[e].x;
+        if (d == 0) {
+          sm.m[0][r] = y[e].top;
+          sm.l[0][r] = y[e].sum;
+        }
+      }
+    }
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    // a row is a stretch of D/4 threads; ranks take rows in turn
+    const int stretch = threadIdx.x / (D / 4), d = (threadIdx.x % (D / 4)) * 4;
+#pragma unroll 1
+    for (int r = rank + stretch * ctas; r < kRows; r += kKaThreads / (D / 4) * ctas) {
+      if (at.rt * kRows + r >= a.rows) break;
+      float top = kNoMax, sum = 0.f;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+      for (int c = 0; c < ctas; ++c) top = fmaxf(top, *cluster.map_shared_rank(&sm.m[0][r], c));
+#pragma unroll 4
+      for (int c = 0; c < ctas; ++c) {
+        const float is = exp2_fast(*cluster.map_shared_rank(&sm.m[0][r], c) - top);
+        const float4 z = *cluster.map_shared_rank(reinterpret_cast<float4*>(&sm.o[0][r][d]), c);
+        x.x += z.x * is; x.y += z.y * is; x.z += z.z * is; x.w += z.w * is;
+        sum += *cluster.map_shared_rank(&sm.l[0][r], c) * is;
+      }
+      write_out(a, at.b, at.h, at.rt * kRows + r, d, x, sum);
+    }
+    cluster.sync();                               // the others may still read this CTA's sums
   }
 
   // out[row][d .. d+3] = x / sum, 0 for a row that saw nothing.
@@ -552,64 +649,91 @@ struct Kv8Attn {
   }
 };
 
-// The line of tiles (below 2^31) in parts of nearly equal length: the first `longer` parts have size + 1
-// tiles, the others size; every part has a tile, and kKaWarps of them while there are that many.
-struct Line {
-  uint32_t parts, size, longer;
-  uint32_t unit, before;           // the unit ((b) or, with lists, (b, h)) that holds this CTA's first tile, and the tiles before it
+__device__ __forceinline__ uint32_t unit_tiles(const Kv8AttnDev& a, int u) {
+  return a.blocks ? kv8_tiles(a, u / a.pg.heads, u % a.pg.heads) : kv8_tiles(a, u, 0);
+}
 
-  __device__ __forceinline__ uint32_t begin(uint32_t c) const { return c * size + min(c, longer); }
-  __device__ __forceinline__ uint32_t part_of(uint32_t x) const {
-    const uint32_t edge = longer * (size + 1);
-    return x < edge ? x / (size + 1) : longer + (x - edge) / size;
-  }
+// Sum of x over the threads before this one, and over all.
+struct Before {
+  uint32_t before, all;
 };
-
-__device__ __forceinline__ Line line_start(const Kv8AttnDev& a, uint32_t* scratch) {
-  // A unit's tiles are those of its segments: all heads and row tiles of b, or all row tiles of (b, h).
-  const int units = a.blocks ? a.pg.batch * a.pg.heads : a.pg.batch;
-  const uint32_t per = a.blocks ? a.row_tiles : a.row_tiles * a.pg.heads;
-  const int each = (units + kKaThreads - 1) / kKaThreads;
-  const int u0 = min((int)threadIdx.x * each, units), u1 = min(u0 + each, units);
-  uint32_t sum = 0;
-  for (int u = u0; u < u1; ++u)
-    sum += per * (a.blocks ? kv8_tiles(a, u / a.pg.heads, u % a.pg.heads) : kv8_tiles(a, u, 0));
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint32_t upto = sum;
+__device__ __forceinline__ Before sum_before(uint32_t x, uint32_t* scratch, int warp, int lane) {
+  uint32_t upto = x;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += x;
+    const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += y;
   }
   if (lane == 31) scratch[warp] = upto;
   __syncthreads();
-  uint32_t total = 0, base = 0;
+  Before r{upto - x, 0};
 #pragma unroll
   for (int w = 0; w < kKaWarps; ++w) {
-    if (w < warp) base += scratch[w];
-    total += scratch[w];
+    if (w < warp) r.before += scratch[w];
+    r.all += scratch[w];
   }
+  return r;
+}
+
+// scratch: 2 * kKaWarps + 2 words.  A thread takes `each` neighbouring units.
+__device__ __forceinline__ Line line_start(const Kv8AttnDev& a, uint32_t* scratch, int warp, int lane) {
+  // A unit's tiles are those of its segments: all heads and row tiles of b, or all row tiles of (b, h).
+  const int units = a.blocks ? a.pg.batch * a.pg.heads : a.pg.batch;
+  const uint32_t per = a.blocks ? a.row_tiles : a.row_tiles * a.pg.heads;
+  const int each = (units - 1) / kKaThreads + 1;
+  const int u0 = min((int)threadIdx.x * each, units), u1 = min(u0 + each, units);
+  uint32_t mine = 0;
+#pragma unroll 1
+  for (int u = u0; u < u1; ++u) mine += per * unit_tiles(a, u);
+  Before tiles = sum_before(mine, scratch, warp, lane);
   Line line{};
-  line.parts = min(gridDim.x, (total + kKaWarps - 1) / kKaWarps);
-  if (line.parts == 0) return line;
-  line.size = total / line.parts;
-  line.longer = total - line.size * line.parts;
-  const uint32_t begin = line.begin(blockIdx.x);
-  uint32_t before = base + upto - sum;
-  if (begin >= before && begin - before < sum) {
-    for (int u = u0; u < u1; ++u) {
-      const uint32_t n = per * (a.blocks ? kv8_tiles(a, u / a.pg.heads, u % a.pg.heads) : kv8_tiles(a, u, 0));
-      if (begin - before < n) {
-        scratch[kKaWarps] = u;
-        scratch[kKaWarps + 1] = before;
+  const uint32_t total = tiles.all;
+  if (total == 0) return line;                          // the whole CTA
+  uint32_t first = tiles.before, count = mine, target;  // in tiles, or in parts
+  if (a.aligned) {
+    line.size = max((total - 1) / (gridDim.x - a.segments) + 1, (uint32_t)kKaWarps);
+    count = 0;
+#pragma unroll 1
+    for (int u = u0; u < u1; ++u) count += per * ((unit_tiles(a, u) + line.size - 1) / line.size);
+    const Before parts = sum_before(count, scratch + kKaWarps, warp, lane);
+    first = parts.before;
+    line.parts = parts.all;
+    target = blockIdx.x;
+  } else {
+    line.parts = min(gridDim.x, (total + kKaWarps - 1) / kKaWarps);
+    line.size = total / line.parts;
+    line.longer = total - line.size * line.parts;
+    target = line.even_begin(blockIdx.x);
+  }
+  if (blockIdx.x >= line.parts) return line;            // the whole CTA
+  if (target >= first && target - first < count) {      // one thread
+    for (int u = u0;; ++u) {
+      const uint32_t n = unit_tiles(a, u);
+      const uint32_t here = per * (a.aligned ? (n + line.size - 1) / line.size : n);
+      if (target - first < here) {
+        scratch[2 * kKaWarps] = u;
+        scratch[2 * kKaWarps + 1] = first;
         break;
       }
-      before += n;
+      first += here;
     }
   }
   __syncthreads();
-  line.unit = scratch[kKaWarps];
-  line.before = scratch[kKaWarps + 1];
+  line.unit = scratch[2 * kKaWarps];
+  line.before = scratch[2 * kKaWarps + 1];
+  if (a.aligned) {
+    // tiles are counted from the unit's first one: the part needs no others
+    const uint32_t n = unit_tiles(a, line.unit);
+    const uint32_t of_segment = (n + line.size - 1) / line.size;
+    const uint32_t seg = (target - line.before) / of_segment, part = (target - line.before) - seg * of_segment;
+    const uint32_t share = n / of_segment, longer = n - share * of_segment;
+    line.begin = seg * n + part * share + min(part, longer);
+    line.end = line.begin + share + (part < longer ? 1 : 0);
+    line.before = 0;
+  } else {
+    line.begin = target;
+    line.end = line.even_begin(blockIdx.x + 1);
+  }
   return line;
 }
 
@@ -618,70 +742,85 @@ __global__ void __launch_bounds__(kKaThreads, D <= 128 && NT == 1 ? 2 : 1) kv8_a
   using K = Kv8Attn<D, NT, E5M2, BF16>;
   extern __shared__ __align__(16) char smem_raw[];
   typename K::Smem& sm = *reinterpret_cast<typename K::Smem*>(smem_raw);
-  __shared__ uint32_t s_line[kKaWarps + 2];
+  __shared__ uint32_t s_line[2 * kKaWarps + 2];
+  __shared__ Place at;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  K k;
-  if (a.whole) {
-    const int rt = blockIdx.x % a.row_tiles, bh = blockIdx.x / a.row_tiles;
-    const int b = bh / a.pg.heads, h = bh % a.pg.heads;
-    const int len = kv8_len(a, b);
-    k.load_q(a, b, h, rt, len, lane);
-    k.stream(a, b, h, len, 0, kv8_tiles(a, b, h), warp, lane);
-    k.finish(a, sm, b, h, rt, -1, warp, lane);
-    return;
-  }
-  const Line line = line_start(a, s_line);
-  if (blockIdx.x < line.parts) {
-    const uint32_t begin = line.begin(blockIdx.x), end = line.begin(blockIdx.x + 1);
-    // segment of `begin`
-    int b, h, rt;
-    uint32_t n = a.blocks ? kv8_tiles(a, line.unit / a.pg.heads, line.unit % a.pg.heads) : kv8_tiles(a, line.unit, 0);
-    const uint32_t seg = (begin - line.before) / n;
-    uint32_t start = line.before + seg * n;           // the segment's first tile on the line
-    rt = (int)(seg % a.row_tiles);
-    if (a.blocks) {
-      b = line.unit / a.pg.heads;
-      h = line.unit % a.pg.heads;
-    } else {
-      b = line.unit;
-      h = (int)(seg / a.row_tiles);
+  // The CTA's place is kept in shared memory: it would cost the tile loop registers.
+  if (a.cluster) {
+    // the CTAs of a cluster share a segment, and need not know the others
+    if (threadIdx.x == 0) {
+      const uint32_t rank = blockIdx.x % a.cluster, seg = blockIdx.x / a.cluster;
+      const int bh = (int)(seg / a.row_tiles);
+      at.rt = (int)(seg % a.row_tiles);
+      at.b = bh / a.pg.heads;
+      at.h = bh - at.b * a.pg.heads;
+      at.n = kv8_tiles(a, at.b, at.h);
+      at.start = 0;
+      const uint32_t share = at.n / a.cluster, longer = at.n - share * a.cluster;
+      at.begin = at.at = rank * share + min(rank, longer);
+      at.end = at.at + share + (rank < longer ? 1 : 0);
     }
-    uint32_t at = begin;
-    for (;;) {
-      const uint32_t first = at - start, last = min(n, end - start);
-      const bool cut = first > 0 || last < n;
-      const int len = kv8_len(a, b);
-      k.load_q(a, b, h, rt, len, lane);
-      k.stream(a, b, h, len, first, last, warp, lane);
-      k.finish(a, sm, b, h, rt, cut ? 2 * (int)blockIdx.x + (at == begin ? 0 : 1) : -1, warp, lane);
-      if (first == 0 && threadIdx.x == 0)
-        a.info[((int64_t)b * a.pg.heads + h) * a.row_tiles + rt] =
-            make_int4((int)blockIdx.x, (int)line.part_of(start + n - 1), at == begin ? 0 : 1, 0);
-      at = start + last;
-      if (at >= end) break;
-      start += n;
-      if (++rt == a.row_tiles) {                      // the next segment that has tiles
-        rt = 0;
-        do {
-          if (++h == a.pg.heads) {
-            h = 0;
-            ++b;
-          }
-          n = kv8_tiles(a, b, h);
-        } while (n == 0);
+  } else {
+    allow_dependents();                               // the merge may be set up from here on; it waits for this grid's end
+    const Line line = line_start(a, s_line, warp, lane);
+    if (blockIdx.x >= line.parts) return;
+    if (threadIdx.x == 0) {
+      at.n = unit_tiles(a, line.unit);
+      const uint32_t seg = (line.begin - line.before) / at.n;
+      at.start = line.before + seg * at.n;
+      at.rt = (int)(seg % a.row_tiles);
+      at.b = a.blocks ? line.unit / a.pg.heads : line.unit;
+      at.h = a.blocks ? line.unit % a.pg.heads : (int)(seg / a.row_tiles);
+      at.begin = at.at = line.begin;
+      at.end = line.end;
+      at.line = line;
+    }
+  }
+  __syncthreads();
+  K k;
+  for (;;) {
+    k.piece(a, sm, at, warp, lane);
+    if (a.cluster > 1) {
+      K::finish_cluster(a, sm, at, blockIdx.x % a.cluster, a.cluster);
+      return;
+    }
+    const uint32_t first = at.at - at.start, last = min(at.n, at.end - at.start);
+    const bool cut = !a.cluster && (first > 0 || last < at.n);
+    K::finish(a, sm, at, cut ? 2 * (int)blockIdx.x + (at.at == at.begin ? 0 : 1) : -1);
+    if (a.cluster) return;
+    const bool done = at.start + last >= at.end;
+    __syncthreads();                                  // the buffers and the place have been read
+    if (threadIdx.x == 0) {
+      if (first == 0)
+        a.info[((int64_t)at.b * a.pg.heads + at.h) * a.row_tiles + at.rt] =
+            make_int4((int)blockIdx.x, (int)at.line.last_part(a.aligned, blockIdx.x, at.start, at.n), at.at == at.begin ? 0 : 1, 0);
+      if (!done) {                                    // the next segment that has tiles
+        at.at = at.start + last;
+        at.start += at.n;
+        if (++at.rt == a.row_tiles) {
+          at.rt = 0;
+          do {
+            if (++at.h == a.pg.heads) {
+              at.h = 0;
+              ++at.b;
+            }
+            at.n = kv8_tiles(a, at.b, at.h);
+          } while (at.n == 0);
+        }
       }
     }
+    if (done) return;
+    __syncthreads();
   }
-  allow_dependents();
 }
 
-// Rows of segments that CTA borders cut, and of segments without tiles.  One CTA per (segment, row):
-// its warps take the parts in turn, each lane D/32 dims.
-constexpr int kKmWarps = 4;
+// Rows of segments of several parts, and of segments without tiles.  One CTA per (segment, row); its warps
+// take the parts in turn, four at a time, each lane D/32 neighbouring dims.
+constexpr int kKmWarps = 8;
 
 template <int D, int NT, bool BF16>
 __global__ void __launch_bounds__(kKmWarps * 32) kv8_merge_kernel(const Kv8AttnDev a) {
-  constexpr int kRows = NT * 8;
+  constexpr int kRows = NT * 8, kPer = D / 32, kAtOnce = 4;
   __shared__ float s_m[kKmWarps], s_l[kKmWarps];
   __shared__ __align__(16) float s_o[kKmWarps][D];
   const int seg = blockIdx.x / kRows, r = blockIdx.x % kRows;
@@ -689,24 +828,50 @@ __global__ void __launch_bounds__(kKmWarps * 32) kv8_merge_kernel(const Kv8AttnD
   const int b = bh / a.pg.heads, h = bh % a.pg.heads;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (rt * kRows + r >= a.rows) return;
-  const bool empty = kv8_tiles(a, b, h) == 0;
   wait_for_previous_grid();
+  const bool empty = kv8_tiles(a, b, h) == 0;
   float top = kNoMax, sum = 0.f;
-  float x[D / 32];
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) x[i] = 0.f;
+  float x[kPer] = {};
   if (!empty) {
     const int4 info = a.info[seg];
     if (info.x == info.y) return;                     // written by its CTA
-    for (int c = info.x + warp; c <= info.y; c += kKmWarps) {
-      const int64_t row = (int64_t)(2 * c + (c == info.x ? info.z : 0)) * kRows + r;
-      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + row * 2);
-      const float m = fmaxf(top, ml.x);
-      const float was = exp2_fast(top - m), is = exp2_fast(ml.x - m);
-      sum = sum * was + ml.y * is;
+#pragma unroll 1
+    for (int c0 = info.x + warp; c0 <= info.y; c0 += kKmWarps * kAtOnce) {
+      float2 ml[kAtOnce];
+      float y[kAtOnce][kPer];
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) x[i] = x[i] * was + a.part_o[row * D + lane + 32 * i] * is;
-      top = m;
+      for (int j = 0; j < kAtOnce; ++j) {
+        const int c = c0 + j * kKmWarps;
+        ml[j] = make_float2(kNoMax, 0.f);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) y[j][i] = 0.f;
+        if (c <= info.y) {
+          const int64_t row = (int64_t)(2 * c + (c == info.x ? info.z : 0)) * kRows + r;
+          ml[j] = *reinterpret_cast<const float2*>(a.part_ml + row * 2);
+          const float* src = a.part_o + row * D + lane * kPer;
+#pragma unroll
+          for (int i = 0; i < kPer; i += 2) {
+            const float2 z = *reinterpret_cast<const float2*>(src + i);
+            y[j][i] = z.x;
+            y[j][i + 1] = z.y;
+          }
+        }
+      }
+      float now = top;
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) now = fmaxf(now, ml[j].x);
+      const float was = exp2_fast(top - now);
+      sum *= was;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) x[i] *= was;
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        const float is = exp2_fast(ml[j].x - now);
+        sum += ml[j].y * is;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) x[i] += y[j][i] * is;
+      }
+      top = now;
     }
   }
   if (lane == 0) {
@@ -714,7 +879,7 @@ __global__ void __launch_bounds__(kKmWarps * 32) kv8_merge_kernel(const Kv8AttnD
     s_l[warp] = sum;
   }
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) s_o[warp][lane + 32 * i] = x[i];
+  for (int i = 0; i < kPer; ++i) s_o[warp][lane * kPer + i] = x[i];
   __syncthreads();
   if (threadIdx.x < D / 4) {
     const int d = threadIdx.x * 4;
@@ -736,7 +901,7 @@ __global__ void __launch_bounds__(kKmWarps * 32) kv8_merge_kernel(const Kv8AttnD
 
 // ---- host --------------------------------------------------------------------------------------
 struct Kv8Plan {
-  int nt, row_tiles, whole;
+  int nt, row_tiles, cluster, aligned;
   int64_t segments, ctas;          // ctas: of the first kernel
   uint64_t info_bytes, ml_bytes, o_bytes;
 };
@@ -748,17 +913,26 @@ static Kv8Plan make_plan(const mskv_kv8_attn_desc& d) {
   p.row_tiles = (rows + p.nt * 8 - 1) / (p.nt * 8);
   p.segments = (int64_t)d.pages.batch * d.pages.kv_heads * p.row_tiles;
   const int64_t most = d.blocks ? (int64_t)d.num_blocks * (d.pages.page_size / 16) : ((int64_t)d.max_tokens + 15) / 16;
-  p.whole = most <= 16;
-  if (p.whole) {
-    p.ctas = p.segments;
+  const int per_sm = d.pages.head_dim <= 128 && p.nt == 1 ? 2 : 1;
+  const int64_t slots = (int64_t)num_sms() * per_sm;      // CTAs that run at once
+  // One cluster a segment, merged in its shared memory: while a warp has up to four tiles, and for lists, which
+  // are of one length as a rule, wherever the clusters fill most of the GPU.  Two tiles a warp decide its size.
+  int cluster = 1;
+  while (cluster < 8 && most > 2 * kKaWarps * cluster && p.segments * cluster * 2 <= slots) cluster *= 2;
+  if (most <= 4 * kKaWarps * cluster || (d.blocks && p.segments <= slots && p.segments * cluster * 5 >= slots * 3)) {
+    p.cluster = cluster;
+    p.ctas = p.segments * cluster;
     return p;
   }
-  const int per_sm = d.pages.head_dim <= 128 && p.nt == 1 ? 2 : 1;
-  p.ctas = std::min<int64_t>((int64_t)num_sms() * per_sm, (p.segments * most + kKaWarps - 1) / kKaWarps);
-  const uint64_t slots = 2 * (uint64_t)p.ctas * p.nt * 8;
+  p.ctas = std::min<int64_t>(slots, (p.segments * most + kKaWarps - 1) / kKaWarps);
+  // Parts that do not cross segments leave CTAs without work (at 128 segments 256 of 296 have some), a part
+  // that does costs a second start.  28/4 heads, 8 sequences of 16384 tokens (111 tiles a CTA): 33.0 us
+  // against 37.1; 40/8 heads, 16 of 32768 (886 a CTA): 199 us against 185.
+  p.aligned = p.segments * 2 <= p.ctas && p.segments * most <= 256 * p.ctas;
+  const uint64_t rows_held = 2 * (uint64_t)p.ctas * p.nt * 8;
   p.info_bytes = ((uint64_t)p.segments * sizeof(int4) + 255) / 256 * 256;
-  p.ml_bytes = (slots * 2 * sizeof(float) + 255) / 256 * 256;
-  p.o_bytes = slots * d.pages.head_dim * sizeof(float);
+  p.ml_bytes = (rows_held * 2 * sizeof(float) + 255) / 256 * 256;
+  p.o_bytes = rows_held * d.pages.head_dim * sizeof(float);
   return p;
 }
 
@@ -767,9 +941,25 @@ static int launch_attn(const Kv8AttnDev& a, const Kv8Plan& p, cudaStream_t st) {
   constexpr int smem = (int)sizeof(typename Kv8Attn<D, NT, E5M2, BF16>::Smem);
   const auto kernel = kv8_attn_kernel<D, NT, E5M2, BF16>;
   if (const int rc = ensure_smem_limit(reinterpret_cast<const void*>(kernel), smem, "mskv_kv8_attention")) return rc;
-  kernel<<<(unsigned)p.ctas, kKaThreads, smem, st>>>(a);
+  if (p.cluster > 1) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)p.ctas);
+    cfg.blockDim = dim3(kKaThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)p.cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+    if (e != cudaSuccess) return cuda_status(e, "mskv_kv8_attention launch");
+  } else {
+    kernel<<<(unsigned)p.ctas, kKaThreads, smem, st>>>(a);
+  }
   if (const int rc = after_launch("mskv_kv8_attention")) return rc;
-  if (p.whole) return MSKV_OK;
+  if (p.cluster) return MSKV_OK;
   const cudaError_t e = launch_dependent(kv8_merge_kernel<D, NT, BF16>, dim3((unsigned)(p.segments * NT * 8)),
                                          dim3(kKmWarps * 32), 0, st, a);
   if (e != cudaSuccess) return cuda_status(e, "mskv_kv8_attention merge launch");
@@ -855,7 +1045,8 @@ extern "C" int mskv_kv8_attention(const mskv_kv8_attn_desc* d, void* stream) {
   a.segments = (int32_t)p.segments;
   a.max_tokens = d->max_tokens;
   a.width = d->num_blocks;
-  a.whole = p.whole;
+  a.cluster = p.cluster;
+  a.aligned = p.aligned;
   a.vec_q = (q_bits & 15) == 0;
   a.pow2_page = (a.pg.page_size & (a.pg.page_size - 1)) == 0;
   const bool e5m2 = d->pages.dtype == MSKV_DT_FP8_E5M2, bf16 = d->dtype == MSKV_DT_BF16;
