@@ -62,8 +62,11 @@ struct Kv8AttnDev {
   int32_t vec_q, pow2_page, aligned;
 };
 
-constexpr int kKaWarps = 8;
-constexpr int kKaThreads = kKaWarps * 32;
+// Warps of a CTA and CTAs of an SM, by what the registers hold: at 64 and 128 dims, up to 8 rows, 128 registers
+// a thread; with a second column tile or 256 dims 168.
+__host__ __device__ constexpr int ka_warps(int d, int nt) { return d == 128 && nt == 2 ? 12 : 8; }
+__host__ __device__ constexpr int ka_ctas(int d, int nt) { return d == 256 || (d == 128 && nt == 2) ? 1 : d == 64 && nt == 1 ? 3 : 2; }
+constexpr int kKaMaxCluster = 8;
 constexpr float kNoMax = -1e30f;
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -98,12 +101,10 @@ __device__ __forceinline__ uint32_t nonfinite_bytes(uint32_t w) {
 // tiles has ceil(n / size) parts of nearly equal length; size = ceil(total / (CTAs - segments))
 // makes them at most as many as the CTAs.  A CTA that starts a second segment starts its pipeline
 // and merges again, about 4 us, which is worth more than the even shares when there are few tiles.
-// Otherwise `parts` parts of nearly equal length, the first `longer` of size + 1 tiles, the others of size.
+// Otherwise all parts are of nearly equal length, the first `longer` of size + 1 tiles, the others of size.
 // Every part has a tile.
 struct Line {
-  uint32_t parts, size, longer;
-  uint32_t begin, end;             // this CTA's tiles
-  uint32_t unit, before;           // the unit ((b) or, with lists, (b, h)) of its first tile, and the tiles before the unit
+  uint32_t size, longer;
 
   __device__ __forceinline__ uint32_t even_begin(uint32_t c) const { return c * size + min(c, longer); }
   // Last part of the segment of tiles [start, start + n) whose first part is c.
@@ -124,6 +125,7 @@ struct Place {
 
 template <int D, int NT, bool E5M2, bool BF16>
 struct Kv8Attn {
+  static constexpr int kWarps = ka_warps(D, NT), kThreads = kWarps * 32;
   static constexpr int kRows = NT * 8;
   static constexpr int kKVec = D / 64;            // 16-byte loads of a lane per K row
   static constexpr int kVWords = D / 32;          // words of a lane per V row
@@ -132,8 +134,8 @@ struct Kv8Attn {
   static constexpr bool kTwoTerms = !BF16;        // P as two fp16 terms
 
   struct Smem {
-    float o[kKaWarps][kRows][kOStride];           // the warps' sums; o[0], m[0] and l[0] then the CTA's
-    float m[kKaWarps][kRows], l[kKaWarps][kRows];
+    float o[kWarps][kRows][kOStride];           // the warps' sums; o[0], m[0] and l[0] then the CTA's
+    float m[kWarps][kRows], l[kWarps][kRows];
     __half q[kRows][D + 8];
     float f[kRows];
     int lim[kRows];                               // tokens that a row sees
@@ -144,52 +146,62 @@ struct Kv8Attn {
   float m[NT][2], l[NT][2];
   float o[NT][kOT][4];
 
-  // Query rows of the segment to shared memory: a warp takes a row (NT of them), a lane D/32 neighbouring
-  // elements, scaled to a largest magnitude in [1, 2).  Row 8*(row tile*NT + nt) + n is position * group + head.
-  static __device__ __forceinline__ void stage_q(const Kv8AttnDev& a, Smem& sm, int b, int h, int rt, int len, int warp, int lane) {
-    constexpr int kPer = D / 32;
-#pragma unroll 1
-    for (int n = warp; n < kRows; n += kKaWarps) {
-      const int r = rt * kRows + n;
-      float x[kPer];
+  // Query rows of the segment to shared memory, in two steps, so that the codes' first loads come between: a
+  // warp takes rows warp and warp + kWarps (two column tiles), a lane D/32 neighbouring elements of each.
+  // Row 8*(row tile*NT + nt) + n is position * group + head.
+  static constexpr int kQEach = (kRows + kWarps - 1) / kWarps, kQPer = D / 32;
+  struct QRows {
+    uint32_t w[kQEach][kQPer / 2];
+  };
+  static __device__ __forceinline__ QRows load_q(const Kv8AttnDev& a, int b, int h, int rt, int warp, int lane) {
+    QRows q;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) x[i] = 0.f;
-      if (r < a.rows) {
+    for (int k = 0; k < kQEach; ++k) {
+      const int n = warp + k * kWarps, r = rt * kRows + n;
+#pragma unroll
+      for (int i = 0; i < kQPer / 2; ++i) q.w[k][i] = 0u;
+      if (n < kRows && r < a.rows) {
         const int pos = r / a.group, head = h * a.group + r - pos * a.group;
-        const char* src = a.q + (int64_t)b * a.q_sb + (int64_t)head * a.q_sh + (int64_t)pos * a.q_sq + lane * (kPer * 2);
-        if (a.vec_q) {
-          uint32_t w[kPer / 2];
-          if constexpr (kPer == 2) {
-            w[0] = *reinterpret_cast<const uint32_t*>(src);
-          } else if constexpr (kPer == 4) {
-            const uint2 y = *reinterpret_cast<const uint2*>(src);
-            w[0] = y.x; w[1] = y.y;
-          } else {
-            const uint4 y = *reinterpret_cast<const uint4*>(src);
-            w[0] = y.x; w[1] = y.y; w[2] = y.z; w[3] = y.w;
-          }
+        const char* src = a.q + (int64_t)b * a.q_sb + (int64_t)head * a.q_sh + (int64_t)pos * a.q_sq + lane * (kQPer * 2);
+        if (!a.vec_q) {
+          const uint16_t* u = reinterpret_cast<const uint16_t*>(src);
 #pragma unroll
-          for (int i = 0; i < kPer; ++i) {
-            const uint16_t u = (uint16_t)(i & 1 ? w[i / 2] >> 16 : w[i / 2]);
-            x[i] = BF16 ? __uint_as_float((uint32_t)u << 16) : __half2float(__ushort_as_half(u));
-          }
+          for (int i = 0; i < kQPer / 2; ++i) q.w[k][i] = (uint32_t)u[2 * i] | ((uint32_t)u[2 * i + 1] << 16);
+        } else if constexpr (kQPer == 2) {
+          q.w[k][0] = *reinterpret_cast<const uint32_t*>(src);
+        } else if constexpr (kQPer == 4) {
+          const uint2 y = *reinterpret_cast<const uint2*>(src);
+          q.w[k][0] = y.x; q.w[k][1] = y.y;
         } else {
-#pragma unroll
-          for (int i = 0; i < kPer; ++i) x[i] = q_elem<BF16>(src + 2 * i);
+          const uint4 y = *reinterpret_cast<const uint4*>(src);
+          q.w[k][0] = y.x; q.w[k][1] = y.y; q.w[k][2] = y.z; q.w[k][3] = y.w;
         }
       }
+    }
+    return q;
+  }
+
+  // Scaled to a largest magnitude in [1, 2), as fp16.
+  static __device__ __forceinline__ void stage_q(const Kv8AttnDev& a, Smem& sm, const QRows& q, int rt, int len, int warp, int lane) {
+#pragma unroll
+    for (int k = 0; k < kQEach; ++k) {
+      const int n = warp + k * kWarps, r = rt * kRows + n;
+      if (n >= kRows) break;
+      float x[kQPer];
       uint32_t top = 0;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const uint32_t u = __float_as_uint(x[i]) & 0x7fffffffu;
-        top = max(top, u < 0x7f800000u ? u : 0u);
+      for (int i = 0; i < kQPer; ++i) {
+        const uint16_t u = (uint16_t)(i & 1 ? q.w[k][i / 2] >> 16 : q.w[k][i / 2]);
+        x[i] = BF16 ? __uint_as_float((uint32_t)u << 16) : __half2float(__ushort_as_half(u));
+        const uint32_t mag = __float_as_uint(x[i]) & 0x7fffffffu;
+        top = max(top, mag < 0x7f800000u ? mag : 0u);
       }
       top = __reduce_max_sync(0xffffffffu, top);
       const int e = top ? min(max((int)(top >> 23) - 127, -120), 120) : 0;
       const float inv = pow2i(-e);
 #pragma unroll
-      for (int i = 0; i < kPer; i += 2)
-        *reinterpret_cast<uint32_t*>(&sm.q[n][lane * kPer + i]) = pack_half2(x[i] * inv, x[i + 1] * inv);
+      for (int i = 0; i < kQPer; i += 2)
+        *reinterpret_cast<uint32_t*>(&sm.q[n][lane * kQPer + i]) = pack_half2(x[i] * inv, x[i + 1] * inv);
       if (lane == 0) {
         sm.f[n] = a.scale_log2 * pow2i(e);
         sm.lim[n] = len - a.q_len + 1 + (r < a.rows ? r / a.group : a.q_len - 1);
@@ -469,7 +481,7 @@ struct Kv8Attn {
       for (int i = 0; i < kVWords; ++i) vr[r][i] &= ~nonfinite_bytes<E5M2>(vr[r][i]);
   }
 
-  // The CTA's tiles of the segment: the warp's share (every kKaWarps-th).  The first tile's codes are on their way
+  // The CTA's tiles of the segment: the warp's share (every kWarps-th).  The first tile's codes are on their way
   // while the query is staged.
   __device__ __forceinline__ void piece(const Kv8AttnDev& a, Smem& sm, const Place& at, int warp, int lane) {
     const int b = at.b, h = at.h, rt = at.rt;
@@ -477,14 +489,15 @@ struct Kv8Attn {
     const int len = kv8_len(a, b);
     const int seen_by_all = len - a.q_len + 1;    // tokens below: every row sees them
     const int mine = first + warp;
-    const int n = mine < last ? (last - mine + kKaWarps - 1) / kKaWarps : 0;
+    const int n = mine < last ? (last - mine + kWarps - 1) / kWarps : 0;
+    const QRows q = load_q(a, b, h, rt, warp, lane);
     // lane j describes this warp's tile 32*k + j; the next 32 are looked up halfway through
     Tile now{-1, 0, 0}, next{-1, 0, 0};
-    if (lane < n) now = find(a, b, h, len, mine + lane * kKaWarps);
+    if (lane < n) now = find(a, b, h, len, mine + lane * kWarps);
     int page = __shfl_sync(0xffffffffu, now.page, 0), tok = __shfl_sync(0xffffffffu, now.tok, 0);
     load_k(a, page, tok, h, len, lane);
     load_v(a, page, tok, h, len, lane);
-    stage_q(a, sm, b, h, rt, len, warp, lane);
+    stage_q(a, sm, q, rt, len, warp, lane);
     __syncthreads();
     start(sm, lane);
 #pragma unroll 1
@@ -492,7 +505,7 @@ struct Kv8Attn {
       if ((i & 31) == 16) {
         const int j = (i & ~31) + 32 + lane;
         next = Tile{-1, 0, 0};
-        if (j < n) next = find(a, at.b, h, len, (int)(at.at - at.start) + warp + j * kKaWarps);
+        if (j < n) next = find(a, at.b, h, len, (int)(at.at - at.start) + warp + j * kWarps);
       }
       const int exps = __shfl_sync(0xffffffffu, now.exps, i & 31);
       if ((i & 31) == 31) now = next;
@@ -539,7 +552,7 @@ struct Kv8Attn {
         const int r = nt * 8 + 2 * c + k;
         float top = sm.m[0][r];
 #pragma unroll
-        for (int w = 1; w < kKaWarps; ++w) top = fmaxf(top, sm.m[w][r]);
+        for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sm.m[w][r]);
         const float down = exp2_fast(m[nt][k] - top);
         // the lane's dims: 128u + (D/8 of them from g on) -- word i of a V row, byte by byte
         constexpr int kPer = D < 128 ? kVWords : 4;
@@ -561,9 +574,9 @@ struct Kv8Attn {
   static __device__ __forceinline__ Part cta_part(const Smem& sm, int r, int d) {
     Part y{make_float4(0.f, 0.f, 0.f, 0.f), sm.m[0][r], 0.f};
 #pragma unroll
-    for (int w = 1; w < kKaWarps; ++w) y.top = fmaxf(y.top, sm.m[w][r]);
+    for (int w = 1; w < kWarps; ++w) y.top = fmaxf(y.top, sm.m[w][r]);
 #pragma unroll
-    for (int w = 0; w < kKaWarps; ++w) {
+    for (int w = 0; w < kWarps; ++w) {
       const float4 z = *reinterpret_cast<const float4*>(&sm.o[w][r][d]);
       y.x.x += z.x; y.x.y += z.y; y.x.z += z.z; y.x.w += z.w;
       y.sum += sm.l[w][r] * exp2_fast(sm.m[w][r] - y.top);
@@ -574,7 +587,7 @@ struct Kv8Attn {
   // Writes the CTA's rows after a piece: to `out`, or (slot >= 0) to the workspace.
   static __device__ __forceinline__ void finish(const Kv8AttnDev& a, const Smem& sm, const Place& at, int slot) {
 #pragma unroll 1
-    for (int i = threadIdx.x; i < kRows * D / 4; i += kKaThreads) {
+    for (int i = threadIdx.x; i < kRows * D / 4; i += kThreads) {
       const int r = i / (D / 4), d = (i % (D / 4)) * 4;
       const Part y = cta_part(sm, r, d);
       if (slot >= 0) {
@@ -589,17 +602,17 @@ struct Kv8Attn {
   // The same for a cluster of `ctas` CTAs that share a segment: every CTA sums its warps in place, then finishes the
   // rows of its rank from all the CTAs' shared memory.
   static __device__ __forceinline__ void finish_cluster(const Kv8AttnDev& a, Smem& sm, const Place& at, int rank, int ctas) {
-    constexpr int kEach = kRows * D / 4 / kKaThreads > 0 ? kRows * D / 4 / kKaThreads : 1;
+    constexpr int kEach = (kRows * D / 4 + kThreads - 1) / kThreads;
     Part y[kEach];
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
-      const int i = threadIdx.x + e * kKaThreads;
+      const int i = threadIdx.x + e * kThreads;
       if (i < kRows * D / 4) y[e] = cta_part(sm, i / (D / 4), (i % (D / 4)) * 4);
     }
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
-      const int i = threadIdx.x + e * kKaThreads, r = i / (D / 4), d = (i % (D / 4)) * 4;
+      const int i = threadIdx.x + e * kThreads, r = i / (D / 4), d = (i % (D / 4)) * 4;
       if (i < kRows * D / 4) {
         *reinterpret_cast<float4*>(&sm.o[0][r][d]) = y[e].x;
         if (d == 0) {
@@ -613,18 +626,31 @@ struct Kv8Attn {
     // a row is a stretch of D/4 threads; ranks take rows in turn
     const int stretch = threadIdx.x / (D / 4), d = (threadIdx.x % (D / 4)) * 4;
 #pragma unroll 1
-    for (int r = rank + stretch * ctas; r < kRows; r += kKaThreads / (D / 4) * ctas) {
+    for (int r = rank + stretch * ctas; r < kRows; r += kThreads / (D / 4) * ctas) {
       if (at.rt * kRows + r >= a.rows) break;
       float top = kNoMax, sum = 0.f;
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-      for (int c = 0; c < ctas; ++c) top = fmaxf(top, *cluster.map_shared_rank(&sm.m[0][r], c));
-#pragma unroll 4
-      for (int c = 0; c < ctas; ++c) {
-        const float is = exp2_fast(*cluster.map_shared_rank(&sm.m[0][r], c) - top);
-        const float4 z = *cluster.map_shared_rank(reinterpret_cast<float4*>(&sm.o[0][r][d]), c);
-        x.x += z.x * is; x.y += z.y * is; x.z += z.z * is; x.w += z.w * is;
-        sum += *cluster.map_shared_rank(&sm.l[0][r], c) * is;
+      // all remote loads at once: one round trip
+      float m[kKaMaxCluster], l[kKaMaxCluster];
+      float4 z[kKaMaxCluster];
+#pragma unroll
+      for (int c = 0; c < kKaMaxCluster; ++c) {
+        m[c] = kNoMax;
+        l[c] = 0.f;
+        z[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (c < ctas) {
+          m[c] = *cluster.map_shared_rank(&sm.m[0][r], c);
+          l[c] = *cluster.map_shared_rank(&sm.l[0][r], c);
+          z[c] = *cluster.map_shared_rank(reinterpret_cast<float4*>(&sm.o[0][r][d]), c);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < kKaMaxCluster; ++c) top = fmaxf(top, m[c]);
+#pragma unroll
+      for (int c = 0; c < kKaMaxCluster; ++c) {
+        const float is = exp2_fast(m[c] - top);
+        x.x += z[c].x * is; x.y += z[c].y * is; x.z += z[c].z * is; x.w += z[c].w * is;
+        sum += l[c] * is;
       }
       write_out(a, at.b, at.h, at.rt * kRows + r, d, x, sum);
     }
@@ -653,96 +679,81 @@ __device__ __forceinline__ uint32_t unit_tiles(const Kv8AttnDev& a, int u) {
   return a.blocks ? kv8_tiles(a, u / a.pg.heads, u % a.pg.heads) : kv8_tiles(a, u, 0);
 }
 
-// Sum of x over the threads before this one, and over all.
-struct Before {
-  uint32_t before, all;
-};
-__device__ __forceinline__ Before sum_before(uint32_t x, uint32_t* scratch, int warp, int lane) {
-  uint32_t upto = x;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += y;
-  }
-  if (lane == 31) scratch[warp] = upto;
-  __syncthreads();
-  Before r{upto - x, 0};
-#pragma unroll
-  for (int w = 0; w < kKaWarps; ++w) {
-    if (w < warp) r.before += scratch[w];
-    r.all += scratch[w];
-  }
-  return r;
-}
-
-// scratch: 2 * kKaWarps + 2 words.  A thread takes `each` neighbouring units.
-__device__ __forceinline__ Line line_start(const Kv8AttnDev& a, uint32_t* scratch, int warp, int lane) {
-  // A unit's tiles are those of its segments: all heads and row tiles of b, or all row tiles of (b, h).
+// The place of this CTA (by one warp, its lanes taking units 32 at a time); false: no part is left for it.
+// A unit's tiles are those of its segments: all heads and row tiles of b, or with lists all row tiles of (b, h).
+template <int kWarps>
+__device__ __forceinline__ bool line_place(const Kv8AttnDev& a, Place& at, int lane) {
   const int units = a.blocks ? a.pg.batch * a.pg.heads : a.pg.batch;
   const uint32_t per = a.blocks ? a.row_tiles : a.row_tiles * a.pg.heads;
-  const int each = (units - 1) / kKaThreads + 1;
-  const int u0 = min((int)threadIdx.x * each, units), u1 = min(u0 + each, units);
-  uint32_t mine = 0;
-#pragma unroll 1
-  for (int u = u0; u < u1; ++u) mine += per * unit_tiles(a, u);
-  Before tiles = sum_before(mine, scratch, warp, lane);
+  const uint32_t n0 = lane < units ? unit_tiles(a, lane) : 0u;
+  uint32_t total = n0;
+#pragma unroll 4
+  for (int u = lane + 32; u < units; u += 32) total += unit_tiles(a, u);
+  total = __reduce_add_sync(0xffffffffu, total) * per;
+  if (total == 0) return false;
   Line line{};
-  const uint32_t total = tiles.all;
-  if (total == 0) return line;                          // the whole CTA
-  uint32_t first = tiles.before, count = mine, target;  // in tiles, or in parts
+  uint32_t target;                 // this CTA's first part, or tile
   if (a.aligned) {
-    line.size = max((total - 1) / (gridDim.x - a.segments) + 1, (uint32_t)kKaWarps);
-    count = 0;
-#pragma unroll 1
-    for (int u = u0; u < u1; ++u) count += per * ((unit_tiles(a, u) + line.size - 1) / line.size);
-    const Before parts = sum_before(count, scratch + kKaWarps, warp, lane);
-    first = parts.before;
-    line.parts = parts.all;
+    line.size = max((total - 1) / (gridDim.x - a.segments) + 1, (uint32_t)kWarps);
     target = blockIdx.x;
   } else {
-    line.parts = min(gridDim.x, (total + kKaWarps - 1) / kKaWarps);
-    line.size = total / line.parts;
-    line.longer = total - line.size * line.parts;
+    const uint32_t parts = min(gridDim.x, (total + kWarps - 1) / kWarps);
+    if (blockIdx.x >= parts) return false;
+    line.size = total / parts;
+    line.longer = total - line.size * parts;
     target = line.even_begin(blockIdx.x);
   }
-  if (blockIdx.x >= line.parts) return line;            // the whole CTA
-  if (target >= first && target - first < count) {      // one thread
-    for (int u = u0;; ++u) {
-      const uint32_t n = unit_tiles(a, u);
-      const uint32_t here = per * (a.aligned ? (n + line.size - 1) / line.size : n);
-      if (target - first < here) {
-        scratch[2 * kKaWarps] = u;
-        scratch[2 * kKaWarps + 1] = first;
-        break;
-      }
-      first += here;
+  uint32_t before = 0;             // parts, or tiles, of the units before
+#pragma unroll 1
+  for (int u0 = 0; u0 < units; u0 += 32) {
+    const int u = u0 + lane;
+    const uint32_t n = u0 == 0 ? n0 : u < units ? unit_tiles(a, u) : 0u;
+    const uint32_t count = per * (a.aligned ? (n + line.size - 1) / line.size : n);
+    uint32_t upto = count;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
     }
+    const uint32_t hit = __ballot_sync(0xffffffffu, before + upto > target);
+    if (hit) {
+      if (lane == __ffs(hit) - 1) {
+        const uint32_t rest = target - (before + upto - count);
+        uint32_t seg;
+        if (a.aligned) {
+          // tiles are counted from the segment's first one: the part needs no others
+          const uint32_t of_segment = (n + line.size - 1) / line.size;
+          seg = rest / of_segment;
+          const uint32_t part = rest - seg * of_segment, share = n / of_segment, longer = n - share * of_segment;
+          at.start = 0;
+          at.at = part * share + min(part, longer);
+          at.end = at.at + share + (part < longer ? 1 : 0);
+        } else {
+          seg = rest / n;
+          at.start = before + upto - count + seg * n;
+          at.at = target;
+          at.end = line.even_begin(blockIdx.x + 1);
+        }
+        at.begin = at.at;
+        at.n = n;
+        at.rt = (int)(seg % a.row_tiles);
+        at.b = a.blocks ? u / a.pg.heads : u;
+        at.h = a.blocks ? u % a.pg.heads : (int)(seg / a.row_tiles);
+        at.line = line;
+      }
+      return true;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
   }
-  __syncthreads();
-  line.unit = scratch[2 * kKaWarps];
-  line.before = scratch[2 * kKaWarps + 1];
-  if (a.aligned) {
-    // tiles are counted from the unit's first one: the part needs no others
-    const uint32_t n = unit_tiles(a, line.unit);
-    const uint32_t of_segment = (n + line.size - 1) / line.size;
-    const uint32_t seg = (target - line.before) / of_segment, part = (target - line.before) - seg * of_segment;
-    const uint32_t share = n / of_segment, longer = n - share * of_segment;
-    line.begin = seg * n + part * share + min(part, longer);
-    line.end = line.begin + share + (part < longer ? 1 : 0);
-    line.before = 0;
-  } else {
-    line.begin = target;
-    line.end = line.even_begin(blockIdx.x + 1);
-  }
-  return line;
+  return false;
 }
 
 template <int D, int NT, bool E5M2, bool BF16>
-__global__ void __launch_bounds__(kKaThreads, D <= 128 && NT == 1 ? 2 : 1) kv8_attn_kernel(const Kv8AttnDev a) {
+__global__ void __launch_bounds__(32 * ka_warps(D, NT), ka_ctas(D, NT)) kv8_attn_kernel(const Kv8AttnDev a) {
   using K = Kv8Attn<D, NT, E5M2, BF16>;
   extern __shared__ __align__(16) char smem_raw[];
   typename K::Smem& sm = *reinterpret_cast<typename K::Smem*>(smem_raw);
-  __shared__ uint32_t s_line[2 * kKaWarps + 2];
+  __shared__ bool s_some;
   __shared__ Place at;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // The CTA's place is kept in shared memory: it would cost the tile loop registers.
@@ -762,21 +773,13 @@ __global__ void __launch_bounds__(kKaThreads, D <= 128 && NT == 1 ? 2 : 1) kv8_a
     }
   } else {
     allow_dependents();                               // the merge may be set up from here on; it waits for this grid's end
-    const Line line = line_start(a, s_line, warp, lane);
-    if (blockIdx.x >= line.parts) return;
-    if (threadIdx.x == 0) {
-      at.n = unit_tiles(a, line.unit);
-      const uint32_t seg = (line.begin - line.before) / at.n;
-      at.start = line.before + seg * at.n;
-      at.rt = (int)(seg % a.row_tiles);
-      at.b = a.blocks ? line.unit / a.pg.heads : line.unit;
-      at.h = a.blocks ? line.unit % a.pg.heads : (int)(seg / a.row_tiles);
-      at.begin = at.at = line.begin;
-      at.end = line.end;
-      at.line = line;
+    if (warp == 0) {
+      const bool some = line_place<K::kWarps>(a, at, lane);
+      if (lane == 0) s_some = some;
     }
   }
   __syncthreads();
+  if (!a.cluster && !s_some) return;
   K k;
   for (;;) {
     k.piece(a, sm, at, warp, lane);
@@ -913,18 +916,18 @@ static Kv8Plan make_plan(const mskv_kv8_attn_desc& d) {
   p.row_tiles = (rows + p.nt * 8 - 1) / (p.nt * 8);
   p.segments = (int64_t)d.pages.batch * d.pages.kv_heads * p.row_tiles;
   const int64_t most = d.blocks ? (int64_t)d.num_blocks * (d.pages.page_size / 16) : ((int64_t)d.max_tokens + 15) / 16;
-  const int per_sm = d.pages.head_dim <= 128 && p.nt == 1 ? 2 : 1;
-  const int64_t slots = (int64_t)num_sms() * per_sm;      // CTAs that run at once
+  const int warps = ka_warps(d.pages.head_dim, p.nt);
+  const int64_t slots = (int64_t)num_sms() * ka_ctas(d.pages.head_dim, p.nt);   // CTAs that run at once
   // One cluster a segment, merged in its shared memory: while a warp has up to four tiles, and for lists, which
   // are of one length as a rule, wherever the clusters fill most of the GPU.  Two tiles a warp decide its size.
   int cluster = 1;
-  while (cluster < 8 && most > 2 * kKaWarps * cluster && p.segments * cluster * 2 <= slots) cluster *= 2;
-  if (most <= 4 * kKaWarps * cluster || (d.blocks && p.segments <= slots && p.segments * cluster * 5 >= slots * 3)) {
+  while (cluster < kKaMaxCluster && most > 2 * warps * cluster && p.segments * cluster * 2 <= slots) cluster *= 2;
+  if (most <= 4 * warps * cluster || (d.blocks && p.segments <= slots && p.segments * cluster * 5 >= slots * 3)) {
     p.cluster = cluster;
     p.ctas = p.segments * cluster;
     return p;
   }
-  p.ctas = std::min<int64_t>(slots, (p.segments * most + kKaWarps - 1) / kKaWarps);
+  p.ctas = std::min<int64_t>(slots, (p.segments * most + warps - 1) / warps);
   // Parts that do not cross segments leave CTAs without work (at 128 segments 256 of 296 have some), a part
   // that does costs a second start.  28/4 heads, 8 sequences of 16384 tokens (111 tiles a CTA): 33.0 us
   // against 37.1; 40/8 heads, 16 of 32768 (886 a CTA): 199 us against 185.
@@ -944,7 +947,7 @@ static int launch_attn(const Kv8AttnDev& a, const Kv8Plan& p, cudaStream_t st) {
   if (p.cluster > 1) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)p.ctas);
-    cfg.blockDim = dim3(kKaThreads);
+    cfg.blockDim = dim3(32 * ka_warps(D, NT));
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
@@ -956,7 +959,7 @@ static int launch_attn(const Kv8AttnDev& a, const Kv8Plan& p, cudaStream_t st) {
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
     if (e != cudaSuccess) return cuda_status(e, "mskv_kv8_attention launch");
   } else {
-    kernel<<<(unsigned)p.ctas, kKaThreads, smem, st>>>(a);
+    kernel<<<(unsigned)p.ctas, 32 * ka_warps(D, NT), smem, st>>>(a);
   }
   if (const int rc = after_launch("mskv_kv8_attention")) return rc;
   if (p.cluster) return MSKV_OK;
