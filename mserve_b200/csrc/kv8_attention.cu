@@ -118,7 +118,7 @@ struct Line {
 // A CTA's place: the segment, its tiles and its first one's place on the line, the CTA's tiles [at, end)
 // from this segment on, its first of all.
 struct Place {
-  int b, h, rt;
+  int b, h, rt, len;
   uint32_t n, start, at, end, begin;
   Line line;
 };
@@ -141,7 +141,9 @@ struct Kv8Attn {
     int lim[kRows];                               // tokens that a row sees
   };
 
-  uint32_t qf[NT][kKVec * 4][2];
+  // With two column tiles the query's fragments stay in shared memory (the registers hold O and the codes).
+  static constexpr bool kKeepQ = NT == 1;
+  uint32_t qf[kKeepQ ? kKVec * 4 : 1][2];
   float f[NT][2];                                 // scale * log2(e) * 2^(row exponent) of the lane's two columns
   float m[NT][2], l[NT][2];
   float o[NT][kOT][4];
@@ -211,16 +213,28 @@ struct Kv8Attn {
 
   // The staged rows as B fragments: column n = lane/4 of column tile nt is row 8*nt + n, the lane's k-steps
   // of a 64-element stretch are its 16 contiguous elements.  Resets the running sums.
+  static __device__ __forceinline__ void q_fragments(const Smem& sm, int nt, int v, int lane, uint32_t (&x)[4][2]) {
+    const uint4* src = reinterpret_cast<const uint4*>(&sm.q[nt * 8 + (lane >> 2)][64 * v + 16 * (lane & 3)]);
+    const uint4 lo = src[0], hi = src[1];
+    x[0][0] = lo.x; x[0][1] = lo.y; x[1][0] = lo.z; x[1][1] = lo.w;
+    x[2][0] = hi.x; x[2][1] = hi.y; x[3][0] = hi.z; x[3][1] = hi.w;
+  }
+
   __device__ __forceinline__ void start(const Smem& sm, int lane) {
-    const int g = lane >> 2, c = lane & 3;
+    const int c = lane & 3;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+      if constexpr (kKeepQ) {
 #pragma unroll
-      for (int v = 0; v < kKVec; ++v) {
-        const uint4* src = reinterpret_cast<const uint4*>(&sm.q[nt * 8 + g][64 * v + 16 * c]);
-        const uint4 x = src[0], y = src[1];
-        qf[nt][v * 4][0] = x.x; qf[nt][v * 4][1] = x.y; qf[nt][v * 4 + 1][0] = x.z; qf[nt][v * 4 + 1][1] = x.w;
-        qf[nt][v * 4 + 2][0] = y.x; qf[nt][v * 4 + 2][1] = y.y; qf[nt][v * 4 + 3][0] = y.z; qf[nt][v * 4 + 3][1] = y.w;
+        for (int v = 0; v < kKVec; ++v) {
+          uint32_t x[4][2];
+          q_fragments(sm, 0, v, lane, x);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            qf[v * 4 + i][0] = x[i][0];
+            qf[v * 4 + i][1] = x[i][1];
+          }
+        }
       }
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
@@ -341,7 +355,7 @@ struct Kv8Attn {
   }
 
   // Scores of the tile in kr; kr is free afterwards.
-  __device__ __forceinline__ void scores(float (&s)[NT][4]) {
+  __device__ __forceinline__ void scores(const Smem& sm, float (&s)[NT][4], int lane) {
     float odd[NT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -351,14 +365,26 @@ struct Kv8Attn {
     for (int v = 0; v < kKVec; ++v) {
       const uint32_t x[4] = {kr[0][v].x, kr[0][v].y, kr[0][v].z, kr[0][v].w};
       const uint32_t y[4] = {kr[1][v].x, kr[1][v].y, kr[1][v].z, kr[1][v].w};
+      uint32_t q[NT][4][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        if constexpr (kKeepQ) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            q[nt][i][0] = qf[v * 4 + i][0];
+            q[nt][i][1] = qf[v * 4 + i][1];
+          }
+        } else {
+          q_fragments(sm, nt, v, lane, q[nt]);
+        }
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         uint32_t a0, a1, a2, a3;
         codes_to_half<E5M2>(x[i], a0, a2);
         codes_to_half<E5M2>(y[i], a1, a3);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          mma_f16((i & 1) ? odd[nt] : s[nt], a0, a1, a2, a3, qf[nt][v * 4 + i][0], qf[nt][v * 4 + i][1]);
+        for (int nt = 0; nt < NT; ++nt) mma_f16((i & 1) ? odd[nt] : s[nt], a0, a1, a2, a3, q[nt][i][0], q[nt][i][1]);
       }
     }
 #pragma unroll
@@ -486,7 +512,7 @@ struct Kv8Attn {
   __device__ __forceinline__ void piece(const Kv8AttnDev& a, Smem& sm, const Place& at, int warp, int lane) {
     const int b = at.b, h = at.h, rt = at.rt;
     const int first = (int)(at.at - at.start), last = (int)min(at.n, at.end - at.start);
-    const int len = kv8_len(a, b);
+    const int len = at.len;
     const int seen_by_all = len - a.q_len + 1;    // tokens below: every row sees them
     const int mine = first + warp;
     const int n = mine < last ? (last - mine + kWarps - 1) / kWarps : 0;
@@ -515,7 +541,7 @@ struct Kv8Attn {
       const bool edge = tok + 16 > seen_by_all;
       float s[NT][4];
       uint32_t p[NT][2], rest[NT][2];
-      if (page >= 0) scores(s);
+      if (page >= 0) scores(sm, s, lane);
       load_k(a, page_ahead, tok_ahead, h, len, lane);
       if (page >= 0) {
         weights(sm, tok, exps, s, p, rest, edge, lane);
@@ -739,6 +765,7 @@ __device__ __forceinline__ bool line_place(const Kv8AttnDev& a, Place& at, int l
         at.rt = (int)(seg % a.row_tiles);
         at.b = a.blocks ? u / a.pg.heads : u;
         at.h = a.blocks ? u % a.pg.heads : (int)(seg / a.row_tiles);
+        at.len = kv8_len(a, at.b);
         at.line = line;
       }
       return true;
@@ -765,6 +792,7 @@ __global__ void __launch_bounds__(32 * ka_warps(D, NT), ka_ctas(D, NT)) kv8_attn
       at.rt = (int)(seg % a.row_tiles);
       at.b = bh / a.pg.heads;
       at.h = bh - at.b * a.pg.heads;
+      at.len = kv8_len(a, at.b);
       at.n = kv8_tiles(a, at.b, at.h);
       at.start = 0;
       const uint32_t share = at.n / a.cluster, longer = at.n - share * a.cluster;
@@ -809,6 +837,7 @@ __global__ void __launch_bounds__(32 * ka_warps(D, NT), ka_ctas(D, NT)) kv8_attn
             }
             at.n = kv8_tiles(a, at.b, at.h);
           } while (at.n == 0);
+          at.len = kv8_len(a, at.b);
         }
       }
     }

@@ -8,6 +8,7 @@ launch), fills the C descriptor and launches on ``torch.cuda.current_stream()``.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 import math
 import weakref
 from dataclasses import dataclass
@@ -17,8 +18,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import (AttnDesc, CopyDesc, FilterDesc, GatherDesc, Kv8AppendDesc, Kv8AttnDesc, Kv8PagesDesc, Kv8ScoreDesc,
-                   Rows, ScoreDesc, TopkDesc, check, lib)
+from ._lib import AttnDesc, CopyDesc, FilterDesc, GatherDesc, Rows, ScoreDesc, TopkDesc, check, lib
 
 _DTYPE_CODE = {
     torch.float32: _lib.DT_F32,
@@ -543,7 +543,6 @@ def image_filter(attn0: torch.Tensor, *, img_start: int, img_seq: int, text_star
 # 8-bit paged KV cache: append, block scores, attention (whole or over selected blocks)
 # ---------------------------------------------------------------------------------------
 KV8_DTYPES = (torch.float8_e4m3fn, torch.float8_e5m2)
-_HALF_DTYPES = (torch.float16, torch.bfloat16)
 
 
 class Kv8Pages(NamedTuple):
@@ -580,53 +579,29 @@ def kv8_pages(num_pages: int, kv_heads: int, head_dim: int, *, page_size: int = 
                     zeros(num_pages, kv_heads, 2, head_dim) if bounds else None)
 
 
-def _fill_kv8(p: Kv8PagesDesc, pages: Kv8Pages, page_table: torch.Tensor, batch: int, device: torch.device) -> None:
-    """Checks the cache's tensors and fills the C description of their addressing."""
-    k, v, exps, bounds = pages
-    if k.dim() != 4 or v.shape != k.shape or k.dtype not in KV8_DTYPES or v.dtype != k.dtype:
-        raise ValueError("k and v must be fp8 [P, Hkv, page, D] of one shape and type")
-    P, H, page, D = k.shape
-    st = k.stride()
-    if st[3] != 1 or st[2] != D or v.stride() != st:
-        raise ValueError("k and v must have contiguous [page, D] pages and the same strides")
-    if exps.dtype != torch.int8 or exps.shape != (P, H, 2) or not exps.is_contiguous():
-        raise ValueError("exps must be a contiguous int8 [P, Hkv, 2] tensor")
-    if bounds is not None and (bounds.dtype != k.dtype or bounds.shape != (P, H, 2, D) or not bounds.is_contiguous()):
-        raise ValueError("bounds must be a contiguous [P, Hkv, 2, D] tensor of the cache's type")
-    if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.shape[0] != batch or page_table.stride(1) != 1:
-        raise ValueError(f"page_table must be int32 [B={batch}, max_pages] with unit inner stride")
-    for t in (k, v, exps, bounds, page_table):
-        if t is not None and t.device != device:
-            raise ValueError(f"the cache and its page table must live on {device}")
-    p.k, p.v, p.exps = k.data_ptr(), v.data_ptr(), exps.data_ptr()
-    if bounds is not None:
-        p.bounds = bounds.data_ptr()
-    p.page_table = page_table.data_ptr()
-    p.stride_page, p.stride_h, p.pt_stride_b = st[0], st[1], page_table.stride(0)
-    p.num_pages, p.max_pages, p.page_size, p.kv_heads, p.head_dim = P, page_table.shape[1], page, H, D
-    p.dtype, p.batch = _DTYPE_CODE[k.dtype], batch
+_kv8_module = None
 
 
-def _kv8_i32(t: torch.Tensor, numel: int, name: str, device: torch.device) -> int:
-    if t.dtype != torch.int32 or t.numel() != numel or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"{name} must be a contiguous int32 tensor of {numel} entries on {device}")
-    return t.data_ptr()
+def _kv8_ext():
+    """The torch binding of mskv_kv8_* (torch_ext/kv8_ops.cpp), loaded once; ImportError with the build command if absent."""
+    global _kv8_module
+    if _kv8_module is None:
+        from . import build
+        path = build.kv8_ext_path()
+        if not path.exists() or not _lib.LIB_PATH.exists():
+            raise ImportError(f"{path} is not built; run `python -m mserve_b200.build`")
+        spec = importlib.util.spec_from_file_location("kv8_ops", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _kv8_module = module
+    return _kv8_module
 
 
-def _kv8_device(t: torch.Tensor, name: str) -> torch.device:
+def _kv8_status(t: torch.Tensor) -> Optional[torch.Tensor]:
     if not t.is_cuda:
-        raise ValueError(f"{name} must be a CUDA tensor")
-    return t.device
-
-
-def _kv8_call(fn, desc, device: torch.device, stream: Optional[torch.cuda.Stream]) -> None:
-    """Launches on `stream` (None: the current stream of the tensors' device), with that device current."""
-    s = stream if stream is not None else torch.cuda.current_stream(device)
-    if device.index == torch.cuda.current_device():
-        check(fn(C.byref(desc), s.cuda_stream))
-    else:
-        with torch.cuda.device(device):
-            check(fn(C.byref(desc), s.cuda_stream))
+        return None                 # the binding refuses the call
+    w = _status.get(t.device.index)
+    return w if w is not None else status_word(t.device)
 
 
 def kv8_append(pages: Kv8Pages, page_table: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, *,
@@ -641,34 +616,10 @@ def kv8_append(pages: Kv8Pages, page_table: torch.Tensor, k_new: torch.Tensor, v
     and its K bounds follow.  Tokens behind the last new one leave the sequence.  The lengths are the
     caller's: the next call's tok0, and `lens` of the calls below.
     """
-    dev = _kv8_device(k_new, "k_new")
-    if k_new.dim() != 4 or v_new.shape != k_new.shape or v_new.dtype != k_new.dtype:
-        raise ValueError("k_new and v_new must be [B, Hkv, n, D] of one shape and type")
-    if k_new.dtype not in COMPUTE_DTYPES:
-        raise TypeError(f"new rows must be float32/float16/bfloat16, got {k_new.dtype}")
-    B, H, n, D = k_new.shape
-    if H != pages.k.shape[1] or D != pages.k.shape[3]:
-        raise ValueError(f"rows [{B}, {H}, {n}, {D}] do not match a cache of {tuple(pages.k.shape)}")
-    if v_new.device != dev:
-        raise ValueError(f"v_new must live on {dev}")
-    ks, vs = k_new.stride(), v_new.stride()
-    if n and (ks[3] != 1 or vs[3] != 1):
-        raise ValueError("the head_dim axis of the rows must be contiguous")
-    d = Kv8AppendDesc()
-    _fill_kv8(d.pages, pages, page_table, B, dev)
-    d.tok0 = _kv8_i32(tok0, B, "tok0", dev)
-    if counts is not None:
-        d.counts = _kv8_i32(counts, B, "counts", dev)
-    if B == 0 or n == 0:
-        return
-    es = k_new.element_size()
-    d.k_new, d.v_new = k_new.data_ptr(), v_new.data_ptr()
-    d.k_stride_b, d.k_stride_h, d.k_stride_t = ks[0] * es, ks[1] * es, ks[2] * es
-    d.v_stride_b, d.v_stride_h, d.v_stride_t = vs[0] * es, vs[1] * es, vs[2] * es
-    if status:
-        d.status = status_word(dev).data_ptr()
-    d.dtype, d.num_tokens = _DTYPE_CODE[k_new.dtype], n
-    _kv8_call(lib().mskv_kv8_append, d, dev, stream)
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return kv8_append(pages, page_table, k_new, v_new, tok0=tok0, counts=counts, status=status)
+    check(_kv8_ext().append(*pages, page_table, k_new, v_new, tok0, counts, _kv8_status(k_new) if status else None))
 
 
 def kv8_block_score(q: torch.Tensor, pages: Kv8Pages, page_table: torch.Tensor, *, lens: torch.Tensor, max_blocks: int,
@@ -682,36 +633,10 @@ def kv8_block_score(q: torch.Tensor, pages: Kv8Pages, page_table: torch.Tensor, 
     the page has a larger GQA-summed q.k.  ops.topk over the rows (len_: blocks per sequence; recent:
     the last blocks) gives the list for kv8_attention.
     """
-    dev = _kv8_device(q, "q")
-    if q.dim() == 4:
-        q = q[:, :, -1, :]
-    if q.dim() != 3 or q.stride(2) != 1:
-        raise ValueError("q must be [B, Hq, D] with contiguous D")
-    if q.dtype not in _HALF_DTYPES:
-        raise TypeError(f"q must be float16 or bfloat16, got {q.dtype}")
-    if pages.bounds is None:
-        raise ValueError("block scores need pages with bounds")
-    B, Hq, D = q.shape
-    H = pages.k.shape[1]
-    if D != pages.k.shape[3] or Hq % H:
-        raise ValueError(f"q {tuple(q.shape)} does not match a cache of {tuple(pages.k.shape)}")
-    if out.dtype != torch.float32 or out.dim() != 3 or out.stride(2) != 1 or out.shape[:2] != (B, H) \
-            or out.shape[2] < max_blocks or out.stride(0) != H * out.stride(1) or out.device != dev:
-        raise ValueError(f"out must be fp32 [B, Hkv, >= max_blocks] on {dev} with rows at a common stride")
-    d = Kv8ScoreDesc()
-    _fill_kv8(d.pages, pages, page_table, B, dev)
-    d.lens = _kv8_i32(lens, B, "lens", dev)
-    if not 0 <= max_blocks <= page_table.shape[1]:
-        raise ValueError(f"max_blocks must lie in [0, {page_table.shape[1]}]")
-    if B == 0 or max_blocks == 0:
-        return out
-    d.q = q.data_ptr()
-    es = q.element_size()
-    d.q_stride_b, d.q_stride_h = q.stride(0) * es, q.stride(1) * es
-    d.scores, d.scores_stride = out.data_ptr(), max(out.stride(1), max_blocks) if B * H == 1 else out.stride(1)
-    d.status = status_word(dev).data_ptr()
-    d.dtype, d.q_heads, d.max_blocks = _DTYPE_CODE[q.dtype], Hq, int(max_blocks)
-    _kv8_call(lib().mskv_kv8_block_score, d, dev, stream)
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return kv8_block_score(q, pages, page_table, lens=lens, max_blocks=max_blocks, out=out)
+    check(_kv8_ext().block_score(q, *pages, page_table, lens, max_blocks, out, _kv8_status(q)))
     return out
 
 
@@ -728,68 +653,12 @@ def kv8_attention(q: torch.Tensor, pages: Kv8Pages, page_table: torch.Tensor, *,
     output), counts: int32 [B, Hkv] entries of them (None: S); a page listed twice counts twice.
     scale: 1/sqrt(D) by default.  Returns [B, Hq, Q, D] in q's dtype.
     """
-    dev = _kv8_device(q, "q")
-    if q.dim() != 4:
-        raise ValueError("q must be [B, Hq, Q, D]")
-    if q.dtype not in _HALF_DTYPES:
-        raise TypeError(f"q must be float16 or bfloat16, got {q.dtype}")
-    B, Hq, Q, D = q.shape
-    H, page = pages.k.shape[1], pages.k.shape[2]
-    if D != pages.k.shape[3] or Hq == 0 or Hq % H:
-        raise ValueError(f"q {tuple(q.shape)} does not match a cache of {tuple(pages.k.shape)}")
-    if not 1 <= Q <= _lib.KV8_MAX_QLEN:
-        raise ValueError(f"q must hold 1 to {_lib.KV8_MAX_QLEN} positions, got {Q}")
-    qs = q.stride()
-    if qs[3] != 1:
-        raise ValueError("q must have a contiguous head_dim")
-    d = Kv8AttnDesc()
-    _fill_kv8(d.pages, pages, page_table, B, dev)
-    d.lens = _kv8_i32(lens, B, "lens", dev)
-    most = page_table.shape[1] * page
-    if max_tokens is None:
-        max_tokens = most
-    elif not 0 <= max_tokens <= most:
-        raise ValueError(f"max_tokens must lie in [0, {most}]")
-    if blocks is not None:
-        if blocks.dtype != torch.int32 or blocks.dim() != 3 or blocks.shape[:2] != (B, H) or blocks.device != dev \
-                or (blocks.shape[2] > 1 and blocks.stride(2) != 1):
-            raise ValueError(f"blocks must be int32 [B={B}, Hkv={H}, S] on {dev} with unit inner stride")
-        if counts is not None:
-            d.counts = _kv8_i32(counts, B * H, "counts", dev)
-        # an empty list has no address, and None means the whole cache
-        d.blocks = blocks.data_ptr() if blocks.numel() else lens.data_ptr()
-        d.blk_stride_b, d.blk_stride_h, d.num_blocks = blocks.stride(0), blocks.stride(1), blocks.shape[2]
-    elif counts is not None:
-        raise ValueError("counts go with blocks")
-    s = stream if stream is not None else torch.cuda.current_stream(dev)
-    if out is not None:
-        if out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(3) != 1:
-            raise ValueError("out must have q's shape, dtype and device and a contiguous head_dim")
-    elif stream is None:
-        out = torch.empty(B, Hq, Q, D, dtype=q.dtype, device=dev)
-    else:
-        with torch.cuda.stream(s):      # the output belongs to the launching stream
-            out = torch.empty(B, Hq, Q, D, dtype=q.dtype, device=dev)
-    if B == 0:
-        return out
-    es, os_ = q.element_size(), out.stride()
-    d.q, d.out = q.data_ptr(), out.data_ptr()
-    d.q_stride_b, d.q_stride_h, d.q_stride_q = qs[0] * es, qs[1] * es, qs[2] * es
-    d.out_stride_b, d.out_stride_h, d.out_stride_q = os_[0] * es, os_[1] * es, os_[2] * es
-    d.status = status_word(dev).data_ptr()
-    d.scale = float(scale) if scale is not None else 1.0 / math.sqrt(D)
-    d.dtype, d.q_heads, d.q_len, d.max_tokens = _DTYPE_CODE[q.dtype], Hq, Q, int(max_tokens)
-    need = int(lib().mskv_kv8_attention_workspace_bytes(C.byref(d)))
-    if need:
-        # a tensor of the call: the allocator keeps its memory from calls on other streams and from
-        # other graphs for as long as this launch can use it
-        if stream is None:
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        else:
-            with torch.cuda.stream(s):
-                ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        d.workspace, d.workspace_bytes = ws.data_ptr(), need
-    _kv8_call(lib().mskv_kv8_attention, d, dev, s)
+    if stream is not None:
+        with torch.cuda.stream(stream):     # outputs and workspace belong to the launching stream
+            return kv8_attention(q, pages, page_table, lens=lens, max_tokens=max_tokens, blocks=blocks, counts=counts,
+                                 scale=scale, out=out)
+    rc, out = _kv8_ext().attention(q, *pages, page_table, lens, max_tokens, blocks, counts, scale, out, _kv8_status(q))
+    check(rc)
     return out
 
 

@@ -125,7 +125,13 @@ def test_workspace(built_lib):
     assert lib.mskv_kv8_attention_workspace_bytes(C.byref(d)) == 0
 
 
-def test_wrapper_refusals(built_lib):
+@pytest.fixture(scope="session")
+def ext(built_lib):
+    from mserve_b200 import build
+    return build.build_kv8_ext()
+
+
+def test_new_pages(built_lib):
     from mserve_b200 import ops
     with pytest.raises(TypeError):
         ops.kv8_pages(4, 2, 128, dtype=torch.float16, device="cpu")
@@ -134,43 +140,80 @@ def test_wrapper_refusals(built_lib):
             ops.kv8_pages(4, 2, **{"head_dim": 128, "device": "cpu", **kw})
     pages = ops.kv8_pages(4, 2, 128, device="cpu")
     assert pages.k.shape == (4, 2, 16, 128) and pages.bounds.shape == (4, 2, 2, 128) and pages.exps.dtype == torch.int8
+    assert not pages.k.view(torch.uint8).any() and pages.k.data_ptr() != pages.v.data_ptr()
     assert ops.kv8_pages(4, 2, 64, device="cpu", bounds=False).bounds is None
-    i32 = torch.zeros(1, dtype=torch.int32)
-    x = torch.zeros(1, 2, 3, 128, dtype=torch.bfloat16)
-    with pytest.raises(ValueError, match="CUDA"):
-        ops.kv8_append(pages, i32.view(1, 1), x, x, tok0=i32)
-    with pytest.raises(ValueError, match="CUDA"):
-        ops.kv8_block_score(x[:, :, 0], pages, i32.view(1, 1), lens=i32, max_blocks=1, out=torch.zeros(1, 2, 1))
-    with pytest.raises(ValueError, match="CUDA"):
-        ops.kv8_attention(x, pages, i32.view(1, 1), lens=i32)
 
 
-def test_descriptions_are_checked(built_lib):
-    """_fill_kv8: every tensor of the cache by shape, type, layout and device."""
-    from mserve_b200 import _lib, ops
-    cpu = torch.device("cpu")
-    pages = ops.kv8_pages(4, 2, 128, device="cpu")
-    table = torch.zeros(3, 5, dtype=torch.int32)
-    p = _lib.Kv8PagesDesc()
-    ops._fill_kv8(p, pages, table, 3, cpu)
-    assert (p.num_pages, p.max_pages, p.page_size, p.kv_heads, p.head_dim, p.batch) == (4, 5, 16, 2, 128, 3)
-    assert p.stride_page == 2 * 16 * 128 and p.stride_h == 16 * 128 and p.pt_stride_b == 5
+def _calls(pages, table, B=1, D=128):
+    """The three operators on CPU tensors; well-formed calls get as far as the device check."""
+    from mserve_b200 import ops
+    n = torch.zeros(B, dtype=torch.int32)
+    x = torch.zeros(B, 2, 3, D, dtype=torch.bfloat16)
+    q = torch.zeros(B, 6, 1, D, dtype=torch.bfloat16)
+    return [lambda **kw: ops.kv8_append(**{**dict(pages=pages, page_table=table, k_new=x, v_new=x, tok0=n), **kw}),
+            lambda **kw: ops.kv8_block_score(**{**dict(q=q, pages=pages, page_table=table, lens=n, max_blocks=1,
+                                                       out=torch.zeros(B, 2, 1)), **kw}),
+            lambda **kw: ops.kv8_attention(**{**dict(q=q, pages=pages, page_table=table, lens=n), **kw})]
+
+
+def test_cpu_tensors_are_refused(ext):
+    from mserve_b200 import ops
+    pages, table = ops.kv8_pages(4, 2, 128, device="cpu"), torch.zeros(1, 5, dtype=torch.int32)
+    for call in _calls(pages, table):
+        with pytest.raises(ValueError, match="CUDA"):
+            call()
+
+
+def test_the_cache_is_checked(ext):
+    """Every tensor of the cache by shape, type and layout."""
+    from mserve_b200 import ops
+    pages, table = ops.kv8_pages(4, 2, 128, device="cpu"), torch.zeros(3, 5, dtype=torch.int32)
     u8 = lambda t: t.view(torch.uint8)  # noqa: E731
     bad = [pages._replace(k=u8(pages.k)), pages._replace(v=pages.v[:2]), pages._replace(v=pages.v.view(torch.float8_e5m2)),
            pages._replace(k=pages.k.transpose(2, 3)), pages._replace(exps=pages.exps[:3]), pages._replace(exps=u8(pages.exps)),
-           pages._replace(bounds=pages.bounds[..., :64]), pages._replace(bounds=u8(pages.bounds)),
-           pages._replace(k=pages.k[:, :, :, ::2], v=pages.v[:, :, :, ::2])]
+           pages._replace(exps=pages.exps[:, :1]), pages._replace(bounds=pages.bounds[..., :64]), pages._replace(bounds=u8(pages.bounds)),
+           pages._replace(k=pages.k[:, :, :, ::2], v=pages.v[:, :, :, ::2]), pages._replace(k=pages.k[0], v=pages.v[0]),
+           pages._replace(exps=pages.exps.transpose(0, 1).contiguous().transpose(0, 1))]
     for b in bad:
-        with pytest.raises(ValueError):
-            ops._fill_kv8(p, b, table, 3, cpu)
-    for t in (table.long(), table[:2], table.t(), table[0]):
-        with pytest.raises(ValueError):
-            ops._fill_kv8(p, pages, t, 3, cpu)
-    with pytest.raises(ValueError, match="live on"):
-        ops._fill_kv8(p, pages, table, 3, torch.device("cuda", 0))
-    for t in (torch.zeros(2, dtype=torch.int32), torch.zeros(3, dtype=torch.int64), torch.zeros(6, dtype=torch.int32)[::2]):
-        with pytest.raises(ValueError):
-            ops._kv8_i32(t, 3, "lens", cpu)
+        for call in _calls(pages, table, B=3):
+            with pytest.raises(ValueError, match="must"):
+                call(pages=b)
+    for t in (table.long(), table[:2], table.t(), table[0], torch.zeros(3, 10, dtype=torch.int32)[:, ::2]):
+        for call in _calls(pages, table, B=3):
+            with pytest.raises(ValueError, match="page_table"):
+                call(page_table=t)
+
+
+def test_the_arguments_are_checked(ext):
+    from mserve_b200 import ops
+    pages, table = ops.kv8_pages(4, 2, 128, device="cpu"), torch.zeros(1, 5, dtype=torch.int32)
+    append, score, attend = _calls(pages, table)
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+    x = torch.zeros(1, 2, 3, 128, dtype=torch.bfloat16)
+    for kw, error in [(dict(v_new=x[:, :, :2]), ValueError), (dict(v_new=x.half()), ValueError), (dict(k_new=x[0], v_new=x[0]), ValueError),
+                      (dict(k_new=x[..., :64], v_new=x[..., :64]), ValueError), (dict(k_new=x[:, :1], v_new=x[:, :1]), ValueError),
+                      (dict(k_new=x.int(), v_new=x.int()), TypeError), (dict(k_new=x.double(), v_new=x.double()), TypeError),
+                      (dict(k_new=x.repeat(1, 1, 1, 2)[..., ::2], v_new=x), ValueError), (dict(tok0=i32(2)), ValueError),
+                      (dict(tok0=torch.zeros(1)), ValueError), (dict(counts=i32(3)), ValueError)]:
+        with pytest.raises(error):
+            append(**kw)
+    q = torch.zeros(1, 6, 1, 128, dtype=torch.bfloat16)
+    for kw, error in [(dict(q=q.float()), TypeError), (dict(q=q[..., :64]), ValueError), (dict(q=q[:, :5]), ValueError),
+                      (dict(q=q[0, 0]), ValueError), (dict(lens=i32(2)), ValueError), (dict(lens=torch.zeros(1)), ValueError),
+                      (dict(q=q.repeat(1, 1, 1, 2)[..., ::2]), ValueError)]:
+        for call in (score, attend):
+            with pytest.raises(error):
+                call(**kw)
+    for kw in (dict(max_blocks=6, out=torch.zeros(1, 2, 9)), dict(max_blocks=-1), dict(max_blocks=2), dict(out=torch.zeros(1, 1, 4)),
+               dict(out=torch.zeros(1, 2, 4).double()), dict(out=torch.zeros(1, 2, 8)[..., ::2]), dict(pages=pages._replace(bounds=None))):
+        with pytest.raises(ValueError, match="max_blocks|out must|bounds"):
+            score(**kw)
+    for kw in (dict(max_tokens=81), dict(max_tokens=-1), dict(q=q.expand(1, 6, 17, 128)), dict(q=q[:, :, :0]), dict(scale=math.inf),
+               dict(scale=math.nan), dict(blocks=i32(1, 2)), dict(blocks=i32(1, 1, 4)), dict(blocks=i32(1, 2, 4).long()),
+               dict(blocks=i32(1, 2, 8)[..., ::2]), dict(counts=i32(1, 2)), dict(blocks=i32(1, 2, 4), counts=i32(1)),
+               dict(out=torch.zeros_like(q).half()), dict(out=torch.zeros(1, 6, 2, 128, dtype=torch.bfloat16))):
+        with pytest.raises(ValueError, match="must|counts go"):
+            attend(**kw)
 
 
 @pytest.mark.parametrize("dtype", [torch.float8_e4m3fn, torch.float8_e5m2])
