@@ -6,10 +6,18 @@
 // code = rn(x * 2^-e).  The multiplication by a power of two is exact, so a code has one
 // rounding; a page whose exponent a later token raises keeps its codes but for f8 subnormals.
 //
-// One CTA per (page, KV head): page_size/16 warps for K and as many for V, each holding 16
-// rows of its half in registers (8 elements of a row per lane and step), so every new row is
-// read once, and the maximum (an integer maximum over the bits of |x|) and the K bounds are
-// taken from registers.  Old rows are stored again only when the exponent changed.
+// A unit is a (page, KV head): page_size/16 warps for K and as many for V, each with 16 rows of its half, 8
+// neighbouring elements of a row per lane and step; a CTA of 8 warps has as many units as fit (one unit
+// of 2 warps a CTA: 16400 CTAs for 2 x 16384 tokens of 8 heads start no faster than 77 us).
+//  * Pages that only receive 16-bit rows (a prompt's) hold them as loaded, packed: every row is
+//    read once; the maximum is an integer maximum over the packed magnitudes, and the
+//    bounds are packed minima and maxima of the inputs, as rounding keeps their order.
+//  * Other pages (a decode token joins old rows; fp32 rows) read their rows twice, the second time
+//    from the caches: first for the maximum and the bounds, then for the codes.  Old rows are
+//    stored again only when the exponent changed.
+#include <algorithm>
+#include <type_traits>
+
 #include "kv8.cuh"
 
 namespace mskv {
@@ -21,45 +29,116 @@ struct AppendDev {
   const int32_t* tok0;
   const int32_t* counts;
   uint32_t* status;
-  int32_t num_tokens, touched;      // touched: pages of a sequence that num_tokens rows can reach
+  int32_t num_tokens, touched, units;   // touched: pages of a sequence that num_tokens rows can reach; units of a CTA
+  int64_t all_units;
 };
 
 enum NewType { kNewBf16 = 0, kNewF16 = 1, kNewF32 = 2 };
+
+// Eight 16-bit elements as four words.
+template <bool VEC>
+__device__ __forceinline__ void load8_packed(const char* p, uint32_t (&w)[4]) {
+  if constexpr (VEC) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+    w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+  } else {
+    const uint16_t* s = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = (uint32_t)s[2 * i] | ((uint32_t)s[2 * i + 1] << 16);
+  }
+}
+
+template <int NT>
+__device__ __forceinline__ void unpack8(const uint32_t (&w)[4], float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (NT == kNewBf16) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
+  }
+}
 
 template <int NT, bool VEC>
 __device__ __forceinline__ void load8(const char* p, float (&x)[8]) {
   if constexpr (NT == kNewF32) {
     if constexpr (VEC) {
-      const uint4 a = ld_stream16(p), b = ld_stream16(p + 16);
-      const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(w[i]);
+      const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+      x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = reinterpret_cast<const float*>(p)[i];
     }
   } else {
     uint32_t w[4];
-    if constexpr (VEC) {
-      const uint4 a = ld_stream16(p);
-      w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
-    } else {
-      const uint16_t* s = reinterpret_cast<const uint16_t*>(p);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = (uint32_t)s[2 * i] | ((uint32_t)s[2 * i + 1] << 16);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (NT == kNewBf16) {
-        x[2 * i] = __uint_as_float(w[i] << 16);
-        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-      } else {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        x[2 * i] = f.x;
-        x[2 * i + 1] = f.y;
-      }
-    }
+    load8_packed<VEC>(p, w);
+    unpack8<NT>(w, x);
   }
+}
+
+// Eight codes as the values they stand for.
+template <bool E5M2>
+__device__ __forceinline__ void load8_codes(const uint8_t* p, float scale, float (&x)[8]) {
+  const uint2 c = *reinterpret_cast<const uint2*>(p);
+  const uint32_t w[2] = {c.x, c.y};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    uint32_t lo, hi;
+    codes_to_half<E5M2>(w[i], lo, hi);
+    const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+    x[4 * i] = u.x * scale; x[4 * i + 1] = u.y * scale; x[4 * i + 2] = v.x * scale; x[4 * i + 3] = v.y * scale;
+  }
+}
+
+template <bool E5M2>
+__device__ __forceinline__ void store_codes(uint8_t* p, const float (&x)[8], float inv) {
+  uint2 c;
+  c.x = to_codes<E5M2>(x[0] * inv, x[1] * inv) | (to_codes<E5M2>(x[2] * inv, x[3] * inv) << 16);
+  c.y = to_codes<E5M2>(x[4] * inv, x[5] * inv) | (to_codes<E5M2>(x[6] * inv, x[7] * inv) << 16);
+  *reinterpret_cast<uint2*>(p) = c;
+}
+
+template <typename H2>
+__device__ __forceinline__ H2 as_pair(uint32_t w) { return *reinterpret_cast<const H2*>(&w); }
+
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// The warps of one half (K or V) of a unit meet at a barrier of their own, as halves need not meet equally often.
+__device__ __forceinline__ void half_barrier(int bar, int parts) {
+  asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(parts * 32) : "memory");
+}
+
+// Maximum over the warps of a half; slots: a word for each.
+__device__ __forceinline__ uint32_t half_max(uint32_t x, uint32_t* slots, int bar, int parts, int part, int lane) {
+  x = __reduce_max_sync(0xffffffffu, x);
+  if (parts > 1) {
+    if (lane == 0) slots[part] = x;
+    half_barrier(bar, parts);
+    for (int i = 0; i < parts; ++i) x = max(x, slots[i]);
+  }
+  return x;
+}
+
+// Smallest e with a <= F * 2^e for the finite fp32 of bits `a`, F = 1.75 * 2^8 or 1.75 * 2^15.
+template <bool E5M2>
+__device__ __forceinline__ int exponent_for(uint32_t a) {
+  if (!a) return MSKV_KV8_EXP_MIN;
+  const int e = (int)(a >> 23) - 127 - (E5M2 ? 15 : 8) + ((a & 0x7fffffu) > 0x600000u);
+  return min(max(e, MSKV_KV8_EXP_MIN), MSKV_KV8_EXP_MAX);
 }
 
 template <int D, bool E5M2, int NT, bool VEC>
@@ -68,173 +147,194 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const AppendDev a) {
   constexpr int kRows = 32 / kLanes;        // rows of a step
   constexpr int kSteps = 16 / kRows;
   constexpr int kElem = NT == kNewF32 ? 4 : 2;
-  __shared__ uint32_t s_max[2][8];
-  __shared__ __half2 s_lo[8][D / 2], s_hi[8][D / 2];
+  __shared__ uint32_t s_max[2][16];
+  __shared__ float s_lo[8][D], s_hi[8][D];
 
-  const int parts = a.pg.page_size / 16;
+  const int parts = a.pg.page_size >> 4;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int kv = warp / parts, part = warp % parts;
-  const int j = blockIdx.x % a.touched;
-  const int bh = blockIdx.x / a.touched;
-  const int b = bh / a.pg.heads, h = bh % a.pg.heads;
+  const int group = warp / (2 * parts), in_group = warp - group * 2 * parts;
+  const int kv = in_group >= parts, part = in_group - kv * parts;
+  const int bar = 1 + 2 * group + kv;       // a barrier for the warps of each half
+  const int64_t unit = (int64_t)blockIdx.x * a.units + group;
+  if (unit >= a.all_units) return;
+  const int bh = (int)(unit / a.touched), j = (int)(unit - (int64_t)bh * a.touched);
+  const int b = bh / a.pg.heads, h = bh - b * a.pg.heads;
 
-  // the page and its rows; every exit before the barriers is taken by the whole CTA
-  const int64_t tok0 = a.tok0[b];
+  // the page and its rows; every exit before the barriers is taken by the whole unit
+  const int tok0 = a.tok0[b];
   const int n = a.counts ? min(max(a.counts[b], 0), a.num_tokens) : a.num_tokens;
   if (n == 0) return;
   if (tok0 < 0) {
-    if (a.status && threadIdx.x == 0) atomicOr(a.status, MSKV_STATUS_DST_OOB);
+    if (a.status && lane == 0) atomicOr(a.status, MSKV_STATUS_DST_OOB);
     return;
   }
-  const int64_t p = tok0 / a.pg.page_size + j;
-  const int64_t t0 = p * a.pg.page_size;
-  const int64_t end = tok0 + n;
+  const int p = tok0 / a.pg.page_size + j;
+  const int64_t t0 = (int64_t)p * a.pg.page_size;
+  const int64_t end = (int64_t)tok0 + n;
   if (t0 >= end) return;
   if (p >= a.pg.max_pages) {
-    if (a.status && threadIdx.x == 0) atomicOr(a.status, MSKV_STATUS_DST_OOB);
+    if (a.status && lane == 0) atomicOr(a.status, MSKV_STATUS_DST_OOB);
     return;
   }
   const int64_t page = a.pg.page_table[(int64_t)b * a.pg.pt_stride + p];
   if (page < 0 || page >= a.pg.num_pages) {
-    if (a.status && threadIdx.x == 0) atomicOr(a.status, MSKV_STATUS_BAD_PAGE);
+    if (a.status && lane == 0) atomicOr(a.status, MSKV_STATUS_BAD_PAGE);
     return;
   }
   uint8_t* const codes = (kv ? a.pg.v : a.pg.k) + page * a.pg.sp + (int64_t)h * a.pg.sh;
   int8_t* const ex = a.pg.exps + (page * a.pg.heads + h) * 2 + kv;
-  const int first_new = (int)max(tok0 - t0, (int64_t)0);                  // rows [0, first_new) are old
+  const int first_new = (int)max((int64_t)tok0 - t0, (int64_t)0);                  // rows [0, first_new) are old
   const int rows = (int)min(end - t0, (int64_t)a.pg.page_size);           // rows [0, rows) are held
   const int e_old = first_new ? *ex : 0;
   const int r0 = part * 16 + lane / kLanes, d0 = (lane % kLanes) * 8;
+  const char* const src = a.x[kv] + (int64_t)b * a.sb[kv] + (int64_t)h * a.sh[kv] + (t0 + r0 - tok0) * a.st[kv] + d0 * kElem;
+  const int64_t step = (int64_t)kRows * a.st[kv];
 
-  float x[kSteps][8];
+  float lo[8], hi[8];                       // of the K rows, for the lane's elements
 #pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
-    const int r = r0 + s * kRows;
-    if (r >= first_new && r < rows) {
-      const char* src = a.x[kv] + (int64_t)b * a.sb[kv] + (int64_t)h * a.sh[kv] + (t0 + r - tok0) * a.st[kv] + d0 * kElem;
-      load8<NT, VEC>(src, x[s]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[s][i] = 0.f;
-    }
+  for (int i = 0; i < 8; ++i) {
+    lo[i] = INFINITY;
+    hi[i] = -INFINITY;
   }
-  if (part * 16 < first_new) {
-    const float f = pow2i(e_old);
+  if (NT != kNewF32 && first_new == 0) {
+    using H2 = std::conditional_t<NT == kNewBf16, __nv_bfloat162, __half2>;
+    constexpr uint32_t kInf = NT == kNewBf16 ? 0x7f80u : 0x7c00u;
+    uint32_t x[kSteps][4];
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[s][i] = 0u;
+      if (r0 + s * kRows < rows) load8_packed<VEC>(src + s * step, x[s]);
+    }
+    H2 most = as_pair<H2>(0u);
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) most = __hmax2_nan(most, __habs2(as_pair<H2>(x[s][i])));
+    uint32_t both = *reinterpret_cast<const uint32_t*>(&most) & 0x7fff7fffu;   // NaN: all ones
+    uint32_t top = half_max(max(both >> 16, both & 0xffffu), s_max[0] + warp - part, bar, parts, part, lane);
+    if (top >= kInf) {                      // infinities or NaN: the maximum of the others
+      both = 0;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t m = x[s][i] & 0x7fff7fffu;
+          both = __vmaxu2(both, m & __vcmpltu2(m, kInf * 0x10001u));
+        }
+      top = half_max(max(both >> 16, both & 0xffffu), s_max[1] + warp - part, bar, parts, part, lane);
+    }
+    const int e = exponent_for<E5M2>(NT == kNewBf16 ? top << 16 : __float_as_uint(__half2float(__ushort_as_half((uint16_t)top))));
+    const float inv = pow2i(-e);
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       const int r = r0 + s * kRows;
-      if (r < first_new) {
-        const uint2 c = *reinterpret_cast<const uint2*>(codes + (int64_t)r * D + d0);
-        const uint32_t w[2] = {c.x, c.y};
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          uint32_t lo, hi;
-          codes_to_half<E5M2>(w[i], lo, hi);
-          const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&lo));
-          const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-          x[s][4 * i] = u.x * f; x[s][4 * i + 1] = u.y * f; x[s][4 * i + 2] = v.x * f; x[s][4 * i + 3] = v.y * f;
-        }
+      if (r < rows) {
+        float f[8];
+        unpack8<NT>(x[s], f);
+        store_codes<E5M2>(codes + (int64_t)r * D + d0, f, inv);
       }
     }
-  }
-
-  // the largest finite magnitude: fp32 magnitudes order as their bits, non-finite ones count as 0
-  uint32_t top = 0;
+    if (part == 0 && lane == 0) *ex = (int8_t)e;
+    if (!a.pg.bounds) return;               // the same for every thread of the launch
+    if (kv == 0) {
+      H2 l2[4], h2[4];
 #pragma unroll
-  for (int s = 0; s < kSteps; ++s)
+      for (int i = 0; i < 4; ++i) {
+        l2[i] = as_pair<H2>(kInf * 0x10001u);
+        h2[i] = as_pair<H2>(kInf * 0x10001u | 0x80008000u);
+      }
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+        if (r0 + s * kRows < rows)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            l2[i] = __hmin2_nan(l2[i], as_pair<H2>(x[s][i]));
+            h2[i] = __hmax2_nan(h2[i], as_pair<H2>(x[s][i]));
+          }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        lo[2 * i] = __low2float(l2[i]) * inv; lo[2 * i + 1] = __high2float(l2[i]) * inv;
+        hi[2 * i] = __low2float(h2[i]) * inv; hi[2 * i + 1] = __high2float(h2[i]) * inv;
+      }
+    }
+  } else {
+    const float f_old = pow2i(e_old);
+    uint32_t top = 0;                       // fp32 magnitudes order as their bits, non-finite ones count as 0
+#pragma unroll 4
+    for (int s = 0; s < kSteps; ++s) {
+      const int r = r0 + s * kRows;
+      if (r >= rows) break;
+      float x[8];
+      if (r < first_new) load8_codes<E5M2>(codes + (int64_t)r * D + d0, f_old, x);
+      else load8<NT, VEC>(src + s * step, x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t u = __float_as_uint(x[i]) & 0x7fffffffu;
+        top = max(top, u < 0x7f800000u ? u : 0u);
+        lo[i] = min_nan(lo[i], x[i]);
+        hi[i] = max_nan(hi[i], x[i]);
+      }
+    }
+    top = half_max(top, s_max[0] + warp - part, bar, parts, part, lane);
+    const int e = exponent_for<E5M2>(top);
+    const float inv = pow2i(-e);
+    const int r_from = first_new && e == e_old ? first_new : 0;
+#pragma unroll 4
+    for (int s = 0; s < kSteps; ++s) {
+      const int r = r0 + s * kRows;
+      if (r >= rows) break;
+      if (r < r_from) continue;
+      float x[8];
+      if (r < first_new) load8_codes<E5M2>(codes + (int64_t)r * D + d0, f_old, x);
+      else load8<NT, VEC>(src + s * step, x);
+      store_codes<E5M2>(codes + (int64_t)r * D + d0, x, inv);
+    }
+    if (part == 0 && lane == 0) *ex = (int8_t)e;
+    if (!a.pg.bounds) return;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const uint32_t u = __float_as_uint(x[s][i]) & 0x7fffffffu;
-      top = max(top, u < 0x7f800000u ? u : 0u);
-    }
-  top = __reduce_max_sync(0xffffffffu, top);
-  if (parts > 1) {
-    if (lane == 0) s_max[kv][part] = top;
-    __syncthreads();
-    for (int i = 0; i < parts; ++i) top = max(top, s_max[kv][i]);
-  }
-  int e = MSKV_KV8_EXP_MIN;
-  if (top) {
-    e = (int)(top >> 23) - 127 - (E5M2 ? 15 : 8) + ((top & 0x7fffffu) > 0x600000u);
-    e = min(max(e, MSKV_KV8_EXP_MIN), MSKV_KV8_EXP_MAX);
-  }
-
-  const float inv = pow2i(-e);
-  const bool keep_old = first_new && e == e_old;
-  __half2 lo[4], hi[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    lo[i] = __half2half2(__ushort_as_half(0x7c00));
-    hi[i] = __half2half2(__ushort_as_half(0xfc00));
-  }
-#pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
-    const int r = r0 + s * kRows;
-    if (r < rows) {
-      uint2 c;
-      c.x = to_codes<E5M2>(x[s][0] * inv, x[s][1] * inv) | (to_codes<E5M2>(x[s][2] * inv, x[s][3] * inv) << 16);
-      c.y = to_codes<E5M2>(x[s][4] * inv, x[s][5] * inv) | (to_codes<E5M2>(x[s][6] * inv, x[s][7] * inv) << 16);
-      if (r >= first_new || !keep_old) *reinterpret_cast<uint2*>(codes + (int64_t)r * D + d0) = c;
-      if (kv == 0) {
-        uint32_t f[4];
-        codes_to_half<E5M2>(c.x, f[0], f[1]);
-        codes_to_half<E5M2>(c.y, f[2], f[3]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const __half2 v = *reinterpret_cast<const __half2*>(&f[i]);
-          lo[i] = __hmin2_nan(lo[i], v);
-          hi[i] = __hmax2_nan(hi[i], v);
-        }
-      }
+      lo[i] *= inv;
+      hi[i] *= inv;
     }
   }
-  if (part == 0 && lane == 0) *ex = (int8_t)e;
 
-  if (!a.pg.bounds) return;                 // the same for every thread of the launch
-  if (kv == 0) {
+  // bounds over the rows of the warp, then of the warps
+  if (kv) return;
 #pragma unroll
-    for (int o = kLanes; o < 32; o <<= 1)
+  for (int o = kLanes; o < 32; o <<= 1)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        lo[i] = __hmin2_nan(lo[i], __shfl_xor_sync(0xffffffffu, lo[i], o));
-        hi[i] = __hmax2_nan(hi[i], __shfl_xor_sync(0xffffffffu, hi[i], o));
-      }
-  }
+    for (int i = 0; i < 8; ++i) {
+      lo[i] = min_nan(lo[i], __shfl_xor_sync(0xffffffffu, lo[i], o));
+      hi[i] = max_nan(hi[i], __shfl_xor_sync(0xffffffffu, hi[i], o));
+    }
   if (parts > 1) {
-    if (kv == 0 && lane < kLanes)
+    const int first = group * parts;
+    if (lane < kLanes)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s_lo[part][d0 / 2 + i] = lo[i];
-        s_hi[part][d0 / 2 + i] = hi[i];
+      for (int i = 0; i < 8; ++i) {
+        s_lo[first + part][d0 + i] = lo[i];
+        s_hi[first + part][d0 + i] = hi[i];
       }
-    __syncthreads();
-    if (kv == 0 && part == 0 && lane < kLanes)
+    half_barrier(bar, parts);
+    if (part == 0 && lane < kLanes)
       for (int q = 1; q < parts; ++q)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          lo[i] = __hmin2_nan(lo[i], s_lo[q][d0 / 2 + i]);
-          hi[i] = __hmax2_nan(hi[i], s_hi[q][d0 / 2 + i]);
+        for (int i = 0; i < 8; ++i) {
+          lo[i] = min_nan(lo[i], s_lo[first + q][d0 + i]);
+          hi[i] = max_nan(hi[i], s_hi[first + q][d0 + i]);
         }
   }
-  if (kv == 0 && part == 0 && lane < kLanes) {
-    // the bounds are codes of the page, so these conversions are exact
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float2 u0 = __half22float2(lo[2 * i]), u1 = __half22float2(lo[2 * i + 1]);
-      const float2 v0 = __half22float2(hi[2 * i]), v1 = __half22float2(hi[2 * i + 1]);
-      w[i] = to_codes<E5M2>(u0.x, u0.y) | (to_codes<E5M2>(u1.x, u1.y) << 16);
-      w[2 + i] = to_codes<E5M2>(v0.x, v0.y) | (to_codes<E5M2>(v1.x, v1.y) << 16);
-    }
+  if (part == 0 && lane < kLanes) {
     uint8_t* const bd = a.pg.bounds + (page * a.pg.heads + h) * 2 * D + d0;
-    *reinterpret_cast<uint2*>(bd) = make_uint2(w[0], w[1]);
-    *reinterpret_cast<uint2*>(bd + D) = make_uint2(w[2], w[3]);
+    store_codes<E5M2>(bd, lo, 1.f);
+    store_codes<E5M2>(bd + D, hi, 1.f);
   }
 }
 
 template <int D, bool E5M2, int NT>
 static int launch_append(const AppendDev& a, bool vec, int64_t ctas, cudaStream_t st) {
-  const int threads = a.pg.page_size / 16 * 64;
+  const int threads = a.units * a.pg.page_size / 16 * 64;
   if (vec) kv8_append_kernel<D, E5M2, NT, true><<<(unsigned)ctas, threads, 0, st>>>(a);
   else kv8_append_kernel<D, E5M2, NT, false><<<(unsigned)ctas, threads, 0, st>>>(a);
   return after_launch("mskv_kv8_append");
@@ -281,7 +381,9 @@ extern "C" int mskv_kv8_append(const mskv_kv8_append_desc* d, void* stream) {
   a.status = d->status;
   a.num_tokens = d->num_tokens;
   a.touched = (int)(((int64_t)d->num_tokens + a.pg.page_size - 2) / a.pg.page_size + 1);
-  const int64_t ctas = (int64_t)a.touched * a.pg.batch * a.pg.heads;
+  a.units = std::max(1, 64 / a.pg.page_size);             // of 2 * page_size/16 warps: 8, or one unit's 6 to 16
+  a.all_units = (int64_t)a.touched * a.pg.batch * a.pg.heads;
+  const int64_t ctas = (a.all_units + a.units - 1) / a.units;
   if (ctas > INT_MAX) return fail(MSKV_ERR_RANGE, "mskv_kv8_append: too many rows for one call");
   const bool vec = ((k_bits | v_bits) & 15) == 0;   // 16-byte loads; other layouts element by element
   const bool e5m2 = d->pages.dtype == MSKV_DT_FP8_E5M2;

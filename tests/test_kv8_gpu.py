@@ -105,6 +105,31 @@ def test_append_special_values(built_lib, dtype):
     assert int(pages.exps[0, 0, 0]) == k8.EXP_MIN and int(pages.exps[1, 0, 0]) == 0 and int(pages.exps[2, 0, 0]) == 1
 
 
+@pytest.mark.parametrize("new", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("page", [16, 64])
+def test_append_infinities_in_one_half(built_lib, new, page):
+    """Infinities and NaN in K or in V alone, in pages of new rows only and in pages that also hold old ones."""
+    from mserve_b200 import ops
+    H, D = 2, 128
+    g = torch.Generator().manual_seed(77)
+    for where in ("k", "v"):
+        table = torch.arange(4, dtype=torch.int32).view(1, 4)
+        pages = ops.kv8_pages(4, H, D, page_size=page)
+        want = _host(pages)
+        tok0 = 0
+        for n in (2 * page - 5, 9, page):
+            rows = {name: torch.randn(1, H, n, D, generator=g) for name in ("k", "v")}
+            rows[where][0, 0, n // 2, 3] = math.inf
+            rows[where][0, 1, n - 1, 5] = -math.inf
+            rows[where][0, 1, 0, 7] = math.nan
+            rows = {name: t.to(new) for name, t in rows.items()}
+            ops.kv8_append(pages, table.cuda(), rows["k"].cuda(), rows["v"].cuda(), tok0=_i32([tok0]))
+            want = k8.append(want, table, rows["k"].double(), rows["v"].double(), [tok0], [n], E4M3)
+            _same(pages, want)
+            tok0 += n
+    ops.check_status(torch.device("cuda"))
+
+
 def test_append_strides_and_rows_behind(built_lib):
     """Token-major, unaligned and broadcast rows; pools inside one allocation; rows behind the end keep their bytes."""
     from mserve_b200 import ops
