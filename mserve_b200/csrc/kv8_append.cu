@@ -29,8 +29,8 @@ struct AppendDev {
   const int32_t* tok0;
   const int32_t* counts;
   uint32_t* status;
-  int32_t num_tokens, touched, units;   // touched: pages of a sequence that num_tokens rows can reach; units of a CTA
-  int64_t all_units;
+  int32_t num_tokens;
+  uint32_t touched, units, all_units;   // touched: pages of a sequence that num_tokens rows can reach; units of a CTA
 };
 
 enum NewType { kNewBf16 = 0, kNewF16 = 1, kNewF32 = 2 };
@@ -63,35 +63,45 @@ __device__ __forceinline__ void unpack8(const uint32_t (&w)[4], float (&x)[8]) {
   }
 }
 
+// Eight elements of row r of a page as loaded: an old row's codes (two words), a new row's elements (four or
+// eight words), nothing.
 template <int NT, bool VEC>
-__device__ __forceinline__ void load8(const char* p, float (&x)[8]) {
-  if constexpr (NT == kNewF32) {
-    if constexpr (VEC) {
-      const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-      x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+__device__ __forceinline__ void load_row(int r, int first_new, int rows, const uint8_t* codes, int d, int d0, const char* src,
+                                         uint32_t (&w)[NT == kNewF32 ? 8 : 4]) {
+  if (r < first_new) {
+    const uint2 c = *reinterpret_cast<const uint2*>(codes + r * d + d0);
+    w[0] = c.x;
+    w[1] = c.y;
+  } else if (r < rows) {
+    if constexpr (NT != kNewF32) {
+      load8_packed<VEC>(src, w);
+    } else if constexpr (VEC) {
+      const uint4 a = __ldg(reinterpret_cast<const uint4*>(src)), b = __ldg(reinterpret_cast<const uint4*>(src) + 1);
+      w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = reinterpret_cast<const float*>(p)[i];
+      for (int i = 0; i < 8; ++i) w[i] = reinterpret_cast<const uint32_t*>(src)[i];
     }
-  } else {
-    uint32_t w[4];
-    load8_packed<VEC>(p, w);
-    unpack8<NT>(w, x);
   }
 }
 
-// Eight codes as the values they stand for.
-template <bool E5M2>
-__device__ __forceinline__ void load8_codes(const uint8_t* p, float scale, float (&x)[8]) {
-  const uint2 c = *reinterpret_cast<const uint2*>(p);
-  const uint32_t w[2] = {c.x, c.y};
+// Their values: of an old row code * scale.
+template <bool E5M2, int NT>
+__device__ __forceinline__ void row_values(bool old, const uint32_t (&w)[NT == kNewF32 ? 8 : 4], float scale, float (&x)[8]) {
+  if (old) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    uint32_t lo, hi;
-    codes_to_half<E5M2>(w[i], lo, hi);
-    const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&lo));
-    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-    x[4 * i] = u.x * scale; x[4 * i + 1] = u.y * scale; x[4 * i + 2] = v.x * scale; x[4 * i + 3] = v.y * scale;
+    for (int i = 0; i < 2; ++i) {
+      uint32_t lo, hi;
+      codes_to_half<E5M2>(w[i], lo, hi);
+      const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+      x[4 * i] = u.x * scale; x[4 * i + 1] = u.y * scale; x[4 * i + 2] = v.x * scale; x[4 * i + 3] = v.y * scale;
+    }
+  } else if constexpr (NT == kNewF32) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(w[i]);
+  } else {
+    unpack8<NT>(w, x);
   }
 }
 
@@ -141,8 +151,11 @@ __device__ __forceinline__ int exponent_for(uint32_t a) {
   return min(max(e, MSKV_KV8_EXP_MIN), MSKV_KV8_EXP_MAX);
 }
 
-template <int D, bool E5M2, int NT, bool VEC>
-__global__ void __launch_bounds__(512) kv8_append_kernel(const AppendDev a) {
+// kFew: few units (see the launch).  Every page's rows then go through fp32 and are loaded together (eight steps;
+// fp32 rows four), whatever registers that takes; otherwise a page of new rows is kept packed and others take
+// four steps at a time, so that 64 registers do and 32 warps fit an SM.
+template <int D, bool E5M2, int NT, bool VEC, bool kFew>
+__global__ void __launch_bounds__(512, !kFew && D <= 128 && NT != kNewF32 ? 2 : 1) kv8_append_kernel(const AppendDev a) {
   constexpr int kLanes = D / 8;             // lanes of a row
   constexpr int kRows = 32 / kLanes;        // rows of a step
   constexpr int kSteps = 16 / kRows;
@@ -155,10 +168,10 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const AppendDev a) {
   const int group = warp / (2 * parts), in_group = warp - group * 2 * parts;
   const int kv = in_group >= parts, part = in_group - kv * parts;
   const int bar = 1 + 2 * group + kv;       // a barrier for the warps of each half
-  const int64_t unit = (int64_t)blockIdx.x * a.units + group;
+  const uint32_t unit = blockIdx.x * a.units + group;
   if (unit >= a.all_units) return;
-  const int bh = (int)(unit / a.touched), j = (int)(unit - (int64_t)bh * a.touched);
-  const int b = bh / a.pg.heads, h = bh - b * a.pg.heads;
+  const uint32_t bh = unit / a.touched, j = unit - bh * a.touched;
+  const int b = (int)(bh / a.pg.heads), h = (int)(bh - b * a.pg.heads);
 
   // the page and its rows; every exit before the barriers is taken by the whole unit
   const int tok0 = a.tok0[b];
@@ -168,7 +181,7 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const AppendDev a) {
     if (a.status && lane == 0) atomicOr(a.status, MSKV_STATUS_DST_OOB);
     return;
   }
-  const int p = tok0 / a.pg.page_size + j;
+  const int p = tok0 / a.pg.page_size + (int)j;
   const int64_t t0 = (int64_t)p * a.pg.page_size;
   const int64_t end = (int64_t)tok0 + n;
   if (t0 >= end) return;
@@ -196,7 +209,7 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const AppendDev a) {
     lo[i] = INFINITY;
     hi[i] = -INFINITY;
   }
-  if (NT != kNewF32 && first_new == 0) {
+  if (NT != kNewF32 && !kFew && first_new == 0) {
     using H2 = std::conditional_t<NT == kNewBf16, __nv_bfloat162, __half2>;
     constexpr uint32_t kInf = NT == kNewBf16 ? 0x7f80u : 0x7c00u;
     uint32_t x[kSteps][4];
@@ -260,35 +273,47 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const AppendDev a) {
     }
   } else {
     const float f_old = pow2i(e_old);
-    uint32_t top = 0;                       // fp32 magnitudes order as their bits, non-finite ones count as 0
-#pragma unroll 4
-    for (int s = 0; s < kSteps; ++s) {
-      const int r = r0 + s * kRows;
-      if (r >= rows) break;
-      float x[8];
-      if (r < first_new) load8_codes<E5M2>(codes + (int64_t)r * D + d0, f_old, x);
-      else load8<NT, VEC>(src + s * step, x);
+    // a batch of steps: their loads, then their values
+    constexpr int kMost = kFew && NT != kNewF32 ? 8 : 4, kBatch = kSteps < kMost ? kSteps : kMost;
+    uint32_t w[kBatch][kElem * 2];
+    const auto load_batch = [&](int s0) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t u = __float_as_uint(x[i]) & 0x7fffffffu;
-        top = max(top, u < 0x7f800000u ? u : 0u);
-        lo[i] = min_nan(lo[i], x[i]);
-        hi[i] = max_nan(hi[i], x[i]);
+      for (int k = 0; k < kBatch; ++k) load_row<NT, VEC>(r0 + (s0 + k) * kRows, first_new, rows, codes, D, d0, src + (s0 + k) * step, w[k]);
+    };
+    uint32_t top = 0;                       // fp32 magnitudes order as their bits, non-finite ones count as 0
+#pragma unroll 1
+    for (int s0 = 0; s0 < kSteps; s0 += kBatch) {
+      load_batch(s0);
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int r = r0 + (s0 + k) * kRows;
+        if (r >= rows) continue;
+        float x[8];
+        row_values<E5M2, NT>(r < first_new, w[k], f_old, x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t u = __float_as_uint(x[i]) & 0x7fffffffu;
+          top = max(top, u < 0x7f800000u ? u : 0u);
+          lo[i] = min_nan(lo[i], x[i]);
+          hi[i] = max_nan(hi[i], x[i]);
+        }
       }
     }
     top = half_max(top, s_max[0] + warp - part, bar, parts, part, lane);
     const int e = exponent_for<E5M2>(top);
     const float inv = pow2i(-e);
     const int r_from = first_new && e == e_old ? first_new : 0;
-#pragma unroll 4
-    for (int s = 0; s < kSteps; ++s) {
-      const int r = r0 + s * kRows;
-      if (r >= rows) break;
-      if (r < r_from) continue;
-      float x[8];
-      if (r < first_new) load8_codes<E5M2>(codes + (int64_t)r * D + d0, f_old, x);
-      else load8<NT, VEC>(src + s * step, x);
-      store_codes<E5M2>(codes + (int64_t)r * D + d0, x, inv);
+#pragma unroll 1
+    for (int s0 = 0; s0 < kSteps; s0 += kBatch) {
+      if constexpr (kSteps > kBatch) load_batch(s0);      // again, from the caches
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int r = r0 + (s0 + k) * kRows;
+        if (r >= rows || r < r_from) continue;
+        float x[8];
+        row_values<E5M2, NT>(r < first_new, w[k], f_old, x);
+        store_codes<E5M2>(codes + r * D + d0, x, inv);
+      }
     }
     if (part == 0 && lane == 0) *ex = (int8_t)e;
     if (!a.pg.bounds) return;
@@ -333,25 +358,26 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const AppendDev a) {
 }
 
 template <int D, bool E5M2, int NT>
-static int launch_append(const AppendDev& a, bool vec, int64_t ctas, cudaStream_t st) {
+static int launch_append(const AppendDev& a, bool vec, bool few, int64_t ctas, cudaStream_t st) {
   const int threads = a.units * a.pg.page_size / 16 * 64;
-  if (vec) kv8_append_kernel<D, E5M2, NT, true><<<(unsigned)ctas, threads, 0, st>>>(a);
-  else kv8_append_kernel<D, E5M2, NT, false><<<(unsigned)ctas, threads, 0, st>>>(a);
+  const auto go = [&](auto kernel) { kernel<<<(unsigned)ctas, threads, 0, st>>>(a); };
+  if (vec) few ? go(kv8_append_kernel<D, E5M2, NT, true, true>) : go(kv8_append_kernel<D, E5M2, NT, true, false>);
+  else few ? go(kv8_append_kernel<D, E5M2, NT, false, true>) : go(kv8_append_kernel<D, E5M2, NT, false, false>);
   return after_launch("mskv_kv8_append");
 }
 
 template <int D, bool E5M2>
-static int append_type(const AppendDev& a, int dtype, bool vec, int64_t ctas, cudaStream_t st) {
+static int append_type(const AppendDev& a, int dtype, bool vec, bool few, int64_t ctas, cudaStream_t st) {
   switch (dtype) {
-    case MSKV_DT_BF16: return launch_append<D, E5M2, kNewBf16>(a, vec, ctas, st);
-    case MSKV_DT_F16: return launch_append<D, E5M2, kNewF16>(a, vec, ctas, st);
-    default: return launch_append<D, E5M2, kNewF32>(a, vec, ctas, st);
+    case MSKV_DT_BF16: return launch_append<D, E5M2, kNewBf16>(a, vec, few, ctas, st);
+    case MSKV_DT_F16: return launch_append<D, E5M2, kNewF16>(a, vec, few, ctas, st);
+    default: return launch_append<D, E5M2, kNewF32>(a, vec, few, ctas, st);
   }
 }
 
 template <int D>
-static int append_cache(const AppendDev& a, bool e5m2, int dtype, bool vec, int64_t ctas, cudaStream_t st) {
-  return e5m2 ? append_type<D, true>(a, dtype, vec, ctas, st) : append_type<D, false>(a, dtype, vec, ctas, st);
+static int append_cache(const AppendDev& a, bool e5m2, int dtype, bool vec, bool few, int64_t ctas, cudaStream_t st) {
+  return e5m2 ? append_type<D, true>(a, dtype, vec, few, ctas, st) : append_type<D, false>(a, dtype, vec, few, ctas, st);
 }
 
 }  // namespace mskv
@@ -380,17 +406,21 @@ extern "C" int mskv_kv8_append(const mskv_kv8_append_desc* d, void* stream) {
   a.counts = d->counts;
   a.status = d->status;
   a.num_tokens = d->num_tokens;
-  a.touched = (int)(((int64_t)d->num_tokens + a.pg.page_size - 2) / a.pg.page_size + 1);
-  a.units = std::max(1, 64 / a.pg.page_size);             // of 2 * page_size/16 warps: 8, or one unit's 6 to 16
-  a.all_units = (int64_t)a.touched * a.pg.batch * a.pg.heads;
-  const int64_t ctas = (a.all_units + a.units - 1) / a.units;
-  if (ctas > INT_MAX) return fail(MSKV_ERR_RANGE, "mskv_kv8_append: too many rows for one call");
+  a.touched = (uint32_t)(((int64_t)d->num_tokens + a.pg.page_size - 2) / a.pg.page_size + 1);
+  const int64_t all = (int64_t)a.touched * a.pg.batch * a.pg.heads;
+  a.all_units = (uint32_t)all;
+  // Units of 2 * page_size/16 warps: up to 8 warps a CTA, but one unit each while every SM has room for them
+  // (a decode token of 8 sequences, 4 heads: 2.7 us against 3.3).
+  const bool few = all <= 4 * (int64_t)num_sms();
+  a.units = few ? 1 : (uint32_t)std::max(1, 64 / a.pg.page_size);
+  const int64_t ctas = (all + a.units - 1) / a.units;
+  if (all > INT_MAX) return fail(MSKV_ERR_RANGE, "mskv_kv8_append: too many rows for one call");
   const bool vec = ((k_bits | v_bits) & 15) == 0;   // 16-byte loads; other layouts element by element
   const bool e5m2 = d->pages.dtype == MSKV_DT_FP8_E5M2;
   const cudaStream_t st = as_stream(stream);
   switch (d->pages.head_dim) {
-    case 64: return append_cache<64>(a, e5m2, d->dtype, vec, ctas, st);
-    case 128: return append_cache<128>(a, e5m2, d->dtype, vec, ctas, st);
-    default: return append_cache<256>(a, e5m2, d->dtype, vec, ctas, st);
+    case 64: return append_cache<64>(a, e5m2, d->dtype, vec, few, ctas, st);
+    case 128: return append_cache<128>(a, e5m2, d->dtype, vec, few, ctas, st);
+    default: return append_cache<256>(a, e5m2, d->dtype, vec, few, ctas, st);
   }
 }

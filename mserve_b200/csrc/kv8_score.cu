@@ -31,36 +31,68 @@ struct BlockScoreDev {
 constexpr int kBsWarps = 8;
 
 template <int D, bool E5M2, bool BF16>
-__global__ void __launch_bounds__(kBsWarps * 32) kv8_block_score_kernel(const BlockScoreDev a) {
+__global__ void __launch_bounds__(kBsWarps * 32, D <= 128 ? 4 : 2) kv8_block_score_kernel(const BlockScoreDev a) {
   constexpr int kVec = D / 32;              // 16-byte loads of a lane per block (64 codes a step of 4 lanes)
   constexpr int kK = 2 * D / 16;            // k-steps
-  __shared__ __half s_w[2][2 * D];          // the two terms of the weights [min | max]
+  __shared__ __align__(16) uint2 s_w[kK][32];   // the weights [min | max] as B fragments
   __shared__ uint32_t s_top[kBsWarps];
 
-  const int bh = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
-  const int b = bh / a.pg.heads, h = bh % a.pg.heads;
+  const int bh = blockIdx.x / a.chunks, chunk = blockIdx.x - bh * a.chunks;
+  const int b = bh / a.pg.heads, h = bh - b * a.pg.heads;
   const int64_t len = min((int64_t)max(a.lens[b], 0), (int64_t)a.max_blocks * a.pg.page_size);
   const int held = (int)((len + a.pg.page_size - 1) / a.pg.page_size);
   const int first = chunk * a.tiles * kBsWarps * 16;
   if (first >= held) return;                // the whole CTA
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int32_t* const table = a.pg.page_table + (int64_t)b * a.pg.pt_stride;
+  // Block j's page: -2 where there is no block, -1 where its page is unmapped.
+  const auto page_of = [&](int j) {
+    if (j >= held) return -2;
+    const int p = table[j];
+    return p >= 0 && p < a.pg.num_pages ? p : -1;
+  };
+  uint4 x[2][kVec];
+  int e[2];
+  const auto load = [&](const int (&page)[2]) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int64_t ph = (int64_t)page[r] * a.pg.heads + h;
+      e[r] = 0;
+#pragma unroll
+      for (int v = 0; v < kVec; ++v) x[r][v] = make_uint4(0u, 0u, 0u, 0u);
+      if (page[r] >= 0) {
+        const uint8_t* src = a.pg.bounds + ph * 2 * D + 16 * c;
+#pragma unroll
+        for (int v = 0; v < kVec; ++v) x[r][v] = ld_stream16(src + 64 * v);
+        e[r] = a.pg.exps[ph * 2];
+      }
+    }
+  };
+  // the first tile's bounds are on their way while the weights are made
+  const int j0 = first + warp * 16 + g;
+  int page[2] = {page_of(j0), page_of(j0 + 8)};
+  load(page);
+
   // weights: sums over the heads, then both terms at a common power of two
   float up = 0.f, down = 0.f;
   const int d = threadIdx.x;
   if (d < D) {
     const char* q = a.q + (int64_t)b * a.q_sb + (int64_t)h * a.group * a.q_sh + d * 2;
+#pragma unroll 8
     for (int i = 0; i < a.group; ++i) {
-      const float x = q_elem<BF16>(q + (int64_t)i * a.q_sh);
+      const float y = q_elem<BF16>(q + (int64_t)i * a.q_sh);
       // a NaN reaches both sums
-      up += x < 0.f ? 0.f : x;
-      down += x > 0.f ? 0.f : x;
+      up += y < 0.f ? 0.f : y;
+      down += y > 0.f ? 0.f : y;
     }
   }
   const uint32_t mu = __float_as_uint(up) & 0x7fffffffu, md = __float_as_uint(down) & 0x7fffffffu;
   uint32_t top = max(mu < 0x7f800000u ? mu : 0u, md < 0x7f800000u ? md : 0u);
   top = __reduce_max_sync(0xffffffffu, top);
   if (lane == 0) s_top[warp] = top;
+  for (int i = threadIdx.x; i < kK * 32; i += kBsWarps * 32)
+    if ((i & 31) >= 8) s_w[i >> 5][i & 31] = make_uint2(0u, 0u);        // columns 2 to 7
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kBsWarps; ++i) top = max(top, s_top[i]);
@@ -71,51 +103,25 @@ __global__ void __launch_bounds__(kBsWarps * 32) kv8_block_score_kernel(const Bl
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const __half first_term = __float2half_rn(w[i]);
-      s_w[0][i * D + d] = first_term;
       const float rest = (w[i] - __half2float(first_term)) * 4096.f;
-      s_w[1][i * D + d] = __float2half_rn(fabsf(w[i]) <= 65504.f ? rest : 0.f);   // 0 beside an infinity or NaN
+      // element 64 v + 16 c' + 4 k + m of [min | max] is in k-step 4 v + k, lane 4 * column + c', half m
+      const int at = i * D + d, v = at >> 6, c1 = (at >> 4) & 3, k = (at >> 2) & 3, m = at & 3;
+      __half* const lane0 = reinterpret_cast<__half*>(&s_w[4 * v + k][c1]);
+      lane0[m] = first_term;
+      lane0[16 + m] = __float2half_rn(fabsf(w[i]) <= 65504.f ? rest : 0.f);   // column 1; 0 beside an infinity or NaN
     }
   }
   __syncthreads();
-  // B fragments: column g (0, 1: the two terms; others zero), k-step (v, i) = codes 64v + 16c + 4i + 0..3
-  uint32_t w0[kK], w1[kK];
-#pragma unroll
-  for (int v = 0; v < kVec; ++v)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint2 x = make_uint2(0u, 0u);
-      if (g < 2) x = *reinterpret_cast<const uint2*>(&s_w[g][64 * v + 16 * c + 4 * i]);
-      w0[v * 4 + i] = x.x;
-      w1[v * 4 + i] = x.y;
-    }
+  const float q_scale = pow2i(eq);
 
+#pragma unroll 1
   for (int t = 0; t < a.tiles; ++t) {
-    const int j0 = first + (t * kBsWarps + warp) * 16;
-    if (j0 >= held) break;
-    const int j[2] = {j0 + g, j0 + g + 8};
-    int page[2];
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      page[r] = -2;                         // no block
-      if (j[r] < held) {
-        const int p = a.pg.page_table[(int64_t)b * a.pg.pt_stride + j[r]];
-        page[r] = p >= 0 && p < a.pg.num_pages ? p : -1;
-      }
-    }
-    uint4 x[2][kVec];
-    int e[2] = {0, 0};
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int64_t ph = (int64_t)page[r] * a.pg.heads + h;
-      if (page[r] >= 0) {
-        const uint8_t* src = a.pg.bounds + ph * 2 * D + 16 * c;
-#pragma unroll
-        for (int v = 0; v < kVec; ++v) x[r][v] = ld_stream16(src + 64 * v);
-        if (c == 0) e[r] = a.pg.exps[ph * 2];
-      } else {
-#pragma unroll
-        for (int v = 0; v < kVec; ++v) x[r][v] = make_uint4(0u, 0u, 0u, 0u);
-      }
+    const int j = j0 + t * kBsWarps * 16;
+    if (j - g >= held) break;
+    int ahead[2] = {-2, -2};
+    if (t + 1 < a.tiles) {
+      ahead[0] = page_of(j + kBsWarps * 16);
+      ahead[1] = page_of(j + kBsWarps * 16 + 8);
     }
     float acc[2][4] = {};                   // two chains of k-steps
 #pragma unroll
@@ -127,20 +133,25 @@ __global__ void __launch_bounds__(kBsWarps * 32) kv8_block_score_kernel(const Bl
         uint32_t a0, a1, a2, a3;
         codes_to_half<E5M2>(lo_rows[i], a0, a2);
         codes_to_half<E5M2>(hi_rows[i], a1, a3);
-        mma_f16(acc[i & 1], a0, a1, a2, a3, w0[v * 4 + i], w1[v * 4 + i]);
+        const uint2 w = s_w[v * 4 + i][lane];
+        mma_f16(acc[i & 1], a0, a1, a2, a3, w.x, w.y);
       }
     }
+    const int was[2] = {page[0], page[1]}, e_was[2] = {e[0], e[1]};
+    page[0] = ahead[0];
+    page[1] = ahead[1];
+    load(page);
     if (c == 0) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        if (page[r] == -2) continue;
+        if (was[r] == -2) continue;
         float s = (acc[0][2 * r] + acc[1][2 * r]) + (acc[0][2 * r + 1] + acc[1][2 * r + 1]) * (1.f / 4096.f);
-        s = s * pow2i(e[r]) * pow2i(eq);
-        if (page[r] < 0) {
+        s = s * pow2i(e_was[r]) * q_scale;
+        if (was[r] < 0) {
           s = __int_as_float(0xff800000);
           if (a.status) atomicOr(a.status, MSKV_STATUS_BAD_PAGE);
         }
-        a.scores[(int64_t)bh * a.stride + j[r]] = s;
+        a.scores[(int64_t)bh * a.stride + j + 8 * r] = s;
       }
     }
   }
