@@ -168,6 +168,8 @@ __global__ void __launch_bounds__(512, !kFew && D <= 128 && NT != kNewF32 ? 2 : 
   const int group = warp / (2 * parts), in_group = warp - group * 2 * parts;
   const int kv = in_group >= parts, part = in_group - kv * parts;
   const int bar = 1 + 2 * group + kv;       // a barrier for the warps of each half
+  wait_for_previous_grid();
+  allow_dependents();
   const uint32_t unit = blockIdx.x * a.units + group;
   if (unit >= a.all_units) return;
   const uint32_t bh = unit / a.touched, j = unit - bh * a.touched;
@@ -360,9 +362,11 @@ __global__ void __launch_bounds__(512, !kFew && D <= 128 && NT != kNewF32 ? 2 : 
 template <int D, bool E5M2, int NT>
 static int launch_append(const AppendDev& a, bool vec, bool few, int64_t ctas, cudaStream_t st) {
   const int threads = a.units * a.pg.page_size / 16 * 64;
-  const auto go = [&](auto kernel) { kernel<<<(unsigned)ctas, threads, 0, st>>>(a); };
+  cudaError_t launched = cudaSuccess;
+  const auto go = [&](auto kernel) { launched = launch_dependent(kernel, dim3((unsigned)ctas), dim3(threads), 0, st, a); };
   if (vec) few ? go(kv8_append_kernel<D, E5M2, NT, true, true>) : go(kv8_append_kernel<D, E5M2, NT, true, false>);
   else few ? go(kv8_append_kernel<D, E5M2, NT, false, true>) : go(kv8_append_kernel<D, E5M2, NT, false, false>);
+  if (launched != cudaSuccess) return cuda_status(launched, "mskv_kv8_append launch");
   return after_launch("mskv_kv8_append");
 }
 

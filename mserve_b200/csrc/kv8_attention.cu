@@ -783,6 +783,8 @@ __global__ void __launch_bounds__(32 * ka_warps(D, NT), ka_ctas(D, NT)) kv8_attn
   __shared__ bool s_some;
   __shared__ Place at;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  wait_for_previous_grid();
+  allow_dependents();              // what follows may be set up from here on; it waits for this grid's end
   // The CTA's place is kept in shared memory: it would cost the tile loop registers.
   if (a.cluster) {
     // the CTAs of a cluster share a segment, and need not know the others
@@ -800,7 +802,6 @@ __global__ void __launch_bounds__(32 * ka_warps(D, NT), ka_ctas(D, NT)) kv8_attn
       at.end = at.at + share + (rank < longer ? 1 : 0);
     }
   } else {
-    allow_dependents();                               // the merge may be set up from here on; it waits for this grid's end
     if (warp == 0) {
       const bool some = line_place<K::kWarps>(a, at, lane);
       if (lane == 0) s_some = some;
@@ -859,8 +860,9 @@ __global__ void __launch_bounds__(kKmWarps * 32) kv8_merge_kernel(const Kv8AttnD
   const int rt = seg % a.row_tiles, bh = seg / a.row_tiles;
   const int b = bh / a.pg.heads, h = bh % a.pg.heads;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (rt * kRows + r >= a.rows) return;
   wait_for_previous_grid();
+  allow_dependents();
+  if (rt * kRows + r >= a.rows) return;
   const bool empty = kv8_tiles(a, b, h) == 0;
   float top = kNoMax, sum = 0.f;
   float x[kPer] = {};
@@ -973,23 +975,21 @@ static int launch_attn(const Kv8AttnDev& a, const Kv8Plan& p, cudaStream_t st) {
   constexpr int smem = (int)sizeof(typename Kv8Attn<D, NT, E5M2, BF16>::Smem);
   const auto kernel = kv8_attn_kernel<D, NT, E5M2, BF16>;
   if (const int rc = ensure_smem_limit(reinterpret_cast<const void*>(kernel), smem, "mskv_kv8_attention")) return rc;
-  if (p.cluster > 1) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)p.ctas);
-    cfg.blockDim = dim3(32 * ka_warps(D, NT));
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)p.cluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
-    if (e != cudaSuccess) return cuda_status(e, "mskv_kv8_attention launch");
-  } else {
-    kernel<<<(unsigned)p.ctas, 32 * ka_warps(D, NT), smem, st>>>(a);
-  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)p.ctas);
+  cfg.blockDim = dim3(32 * ka_warps(D, NT));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)std::max(p.cluster, 1);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.cluster > 1 ? 2 : 1;
+  const cudaError_t launched = cudaLaunchKernelEx(&cfg, kernel, a);
+  if (launched != cudaSuccess) return cuda_status(launched, "mskv_kv8_attention launch");
   if (const int rc = after_launch("mskv_kv8_attention")) return rc;
   if (p.cluster) return MSKV_OK;
   const cudaError_t e = launch_dependent(kv8_merge_kernel<D, NT, BF16>, dim3((unsigned)(p.segments * NT * 8)),

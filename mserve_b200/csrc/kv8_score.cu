@@ -37,6 +37,8 @@ __global__ void __launch_bounds__(kBsWarps * 32, D <= 128 ? 4 : 2) kv8_block_sco
   __shared__ __align__(16) uint2 s_w[kK][32];   // the weights [min | max] as B fragments
   __shared__ uint32_t s_top[kBsWarps];
 
+  wait_for_previous_grid();
+  allow_dependents();
   const int bh = blockIdx.x / a.chunks, chunk = blockIdx.x - bh * a.chunks;
   const int b = bh / a.pg.heads, h = bh - b * a.pg.heads;
   const int64_t len = min((int64_t)max(a.lens[b], 0), (int64_t)a.max_blocks * a.pg.page_size);
@@ -159,8 +161,9 @@ __global__ void __launch_bounds__(kBsWarps * 32, D <= 128 ? 4 : 2) kv8_block_sco
 
 template <int D, bool E5M2>
 static int launch_block_score(const BlockScoreDev& a, bool bf16, int64_t ctas, cudaStream_t st) {
-  if (bf16) kv8_block_score_kernel<D, E5M2, true><<<(unsigned)ctas, kBsWarps * 32, 0, st>>>(a);
-  else kv8_block_score_kernel<D, E5M2, false><<<(unsigned)ctas, kBsWarps * 32, 0, st>>>(a);
+  const cudaError_t e = launch_dependent(bf16 ? kv8_block_score_kernel<D, E5M2, true> : kv8_block_score_kernel<D, E5M2, false>,
+                                         dim3((unsigned)ctas), dim3(kBsWarps * 32), 0, st, a);
+  if (e != cudaSuccess) return cuda_status(e, "mskv_kv8_block_score launch");
   return after_launch("mskv_kv8_block_score");
 }
 
