@@ -14,14 +14,13 @@
 //    kAtTile = 128 rows (attn_mma_kernel), the splits' (m, l, O) partials in a workspace merged
 //    by a second kernel, one block per (segment, query row).
 // Other shapes use a one-warp-per-output-row kernel with an online softmax.
-#include <cuda.h>   // CUtensorMap and its enums; the encoder is reached through the runtime
 #include <math.h>
 
 #include <algorithm>
-#include <mutex>
 #include <type_traits>
 
 #include "common.cuh"
+#include "tensor_map.cuh"
 
 namespace mskv {
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
@@ -958,26 +957,6 @@ static int64_t splits_of(const mskv_attn_desc* d) {
 }
 
 // ---- streaming cluster path: tensor maps and the split -------------------------------------
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-// cuTensorMapEncodeTiled through the runtime's driver entry point (the library links only the
-// runtime); nullptr when the driver does not offer it.
-static EncodeTiledFn tensor_map_encoder() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(f);
-    cudaGetLastError();
-  });
-  return fn;
-}
-
 // K or V rows as a 3-D tensor [segment][row][dim] of 16-bit elements with 16-row x 64-element
 // boxes and the 128-byte swizzle; rows past the width read as zeros.
 static bool encode_rows_map(CUtensorMap* m, const void* base, const mskv_attn_desc* d) {

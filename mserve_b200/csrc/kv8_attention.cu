@@ -38,6 +38,7 @@
 #include <algorithm>
 
 #include "kv8.cuh"
+#include "tensor_map.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -65,6 +66,7 @@ struct Kv8AttnDev {
 // Warps of a CTA and CTAs of an SM, by what the registers hold: at 64 and 128 dims, up to 8 rows, 128 registers
 // a thread; with a second column tile or 256 dims 168.
 __host__ __device__ constexpr int ka_warps(int d, int nt) { return d == 128 && nt == 2 ? 12 : 8; }
+__host__ __device__ constexpr int ka_stages(int d, int nt) { return d == 64 ? (nt == 1 ? 4 : 6) : d == 128 && nt == 2 ? 4 : 3; }
 __host__ __device__ constexpr int ka_ctas(int d, int nt) { return d == 256 || (d == 128 && nt == 2) ? 1 : d == 64 && nt == 1 ? 3 : 2; }
 constexpr int kKaMaxCluster = 8;
 constexpr float kNoMax = -1e30f;
@@ -133,8 +135,16 @@ struct Kv8Attn {
   static constexpr int kOStride = D + 4;          // floats between rows of the merge buffer
   static constexpr bool kTwoTerms = !BF16;        // P as two fp16 terms
 
+  static constexpr int kBox = 16 * (D < 128 ? D : 128);    // bytes of a box: 16 rows, at most 128 dims
+  static constexpr int kTileBytes = 2 * 16 * D;            // K boxes, then V boxes
+  static constexpr int kStages = ka_stages(D, NT);         // tiles of a warp in flight
+
   struct Smem {
-    float o[kWarps][kRows][kOStride];           // the warps' sums; o[0], m[0] and l[0] then the CTA's
+    union {
+      uint8_t ring[kWarps][kStages][kTileBytes];  // 1024-byte aligned stages (the swizzle's period)
+      float o[kWarps][kRows][kOStride];           // the warps' sums, when the ring is empty; o[0], m[0], l[0] then the CTA's
+    };
+    uint64_t arrived[kWarps][kStages];            // mbarriers
     float m[kWarps][kRows], l[kWarps][kRows];
     __half q[kRows][D + 8];
     float f[kRows];
@@ -282,64 +292,67 @@ struct Kv8Attn {
     return t;
   }
 
-  uint4 kr[2][kKVec];                             // K rows lane/4 and lane/4 + 8
-  uint32_t vr[4][kVWords];                        // V rows 2c, 2c+1, 2c+8, 2c+9
-
-  // Row of the page that a tile begins with.
-  static __device__ __forceinline__ int64_t tile_offset(const Kv8AttnDev& a, int page, int tok, int h) {
-    const int row = a.pow2_page ? tok & (a.pg.page_size - 1) : tok % a.pg.page_size;
-    return (int64_t)page * a.pg.sp + (int64_t)h * a.pg.sh + row * D;
+  // A tile's codes are 16-row boxes in shared memory, their 16-byte chunks permuted by the row (TMA's 128-byte
+  // swizzle, 64-byte at 64 dims).  Fragment row g of K is row g ^ 4*(g & 1) of the tile, so that the eight lanes
+  // of a phase of a 16-byte load read different banks; the tokens of V, the same contraction index, follow.
+  static __device__ __forceinline__ int tile_row(int g) { return g ^ ((g & 1) << 2); }
+  static __device__ __forceinline__ uint32_t chunk_at(int row, int chunk) {
+    return D < 128 ? row * 64 + ((chunk ^ (row >> 1)) & 3) * 16 : row * 128 + (chunk ^ (row & 7)) * 16;
+  }
+  static __device__ __forceinline__ uint4 read16(uint32_t at) {
+    uint4 x;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(at) : "memory");
+    return x;
   }
 
-  // A tile whose 16 tokens all exist is loaded without tests; missing rows are zero.
-  __device__ __forceinline__ void load_k(const Kv8AttnDev& a, int page, int tok, int h, int len, int lane) {
-    if (page < 0) return;
+  // 64 dims of K rows lane/4 and lane/4 + 8: four k-steps.
+  static __device__ __forceinline__ void read_k(uint32_t tile, int v, int lane, uint4 (&x)[2]) {
+    const int row = tile_row(lane >> 2), c = lane & 3;
+    const uint32_t at = tile + (v >> 1) * kBox + chunk_at(row, c + 4 * (v & 1));
+    x[0] = read16(at);
+    x[1] = read16(at + 8 * (D < 128 ? 64 : 128));
+  }
+
+  // V rows of tokens 2c, 2c+1, 2c+8, 2c+9 (as fragment rows), the lane's dims.
+  uint32_t vr[4][kVWords];
+  __device__ __forceinline__ void read_v(uint32_t tile, int lane) {
     const int g = lane >> 2, c = lane & 3;
-    const uint8_t* src = a.pg.k + tile_offset(a, page, tok, h) + g * D + 16 * c;
-    if (tok + 16 <= len) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r)
+    for (int r = 0; r < 4; ++r) {
+      const int row = tile_row(2 * c + (r & 1));
+      const uint32_t at = tile + 16 * D + (r >> 1) * 8 * (D < 128 ? 64 : 128);
+      if constexpr (D == 64) {
+        asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];"
+                     : "=r"(vr[r][0]), "=r"(vr[r][1]) : "r"(at + chunk_at(row, g >> 1) + (g & 1) * 8) : "memory");
+      } else {
 #pragma unroll
-        for (int v = 0; v < kKVec; ++v) kr[r][v] = ld_stream16(src + 8 * r * D + 64 * v);
-    } else {
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-#pragma unroll
-        for (int v = 0; v < kKVec; ++v) {
-          kr[r][v] = make_uint4(0u, 0u, 0u, 0u);
-          if (tok + g + 8 * r < len) kr[r][v] = ld_stream16(src + 8 * r * D + 64 * v);
+        for (int u = 0; u < D / 128; ++u) {
+          const uint4 x = read16(at + u * kBox + chunk_at(row, g));
+          vr[r][4 * u] = x.x; vr[r][4 * u + 1] = x.y; vr[r][4 * u + 2] = x.z; vr[r][4 * u + 3] = x.w;
         }
-    }
-  }
-
-  __device__ __forceinline__ void load_v_row(int r, const uint8_t* src) {
-    if constexpr (D == 64) {
-      const uint2 x = ld_stream8(src);
-      vr[r][0] = x.x; vr[r][1] = x.y;
-    } else {
-#pragma unroll
-      for (int u = 0; u < D / 128; ++u) {
-        const uint4 x = ld_stream16(src + 128 * u);
-        vr[r][4 * u] = x.x; vr[r][4 * u + 1] = x.y; vr[r][4 * u + 2] = x.z; vr[r][4 * u + 3] = x.w;
       }
     }
   }
 
-  __device__ __forceinline__ void load_v(const Kv8AttnDev& a, int page, int tok, int h, int len, int lane) {
-    if (page < 0) return;
-    const int g = lane >> 2, c = lane & 3;
-    const uint8_t* src = a.pg.v + tile_offset(a, page, tok, h) + 2 * c * D + g * (D == 64 ? 8 : 16);
-    if (tok + 16 <= len) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) load_v_row(r, src + ((r >> 1) * 8 + (r & 1)) * D);
-    } else {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-#pragma unroll
-        for (int i = 0; i < kVWords; ++i) vr[r][i] = 0u;
-        if (tok + 2 * c + (r >> 1) * 8 + (r & 1) < len) load_v_row(r, src + ((r >> 1) * 8 + (r & 1)) * D);
-      }
+  // Starts the loads of a tile into a stage (one lane); a tile without tokens completes at once.
+  static __device__ __forceinline__ void fetch(const Kv8AttnDev& a, const CUtensorMap* k_map, const CUtensorMap* v_map, int page,
+                                               int tok, int h, uint32_t stage, uint32_t bar) {
+    if (page < 0) {
+      asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+      return;
     }
+    const int row = a.pow2_page ? tok & (a.pg.page_size - 1) : tok % a.pg.page_size;
+    mbar_expect_tx(bar, kTileBytes);
+#pragma unroll
+    for (int u = 0; u < (D < 128 ? 1 : D / 128); ++u) {
+      load_box(stage + u * kBox, k_map, 128 * u, row, h, page, bar);
+      load_box(stage + 16 * D + u * kBox, v_map, 128 * u, row, h, page, bar);
+    }
+  }
+  static __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int d, int row, int h, int page,
+                                                  uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 ::"r"(dst), "l"(map), "r"(d), "r"(row), "r"(h), "r"(page), "r"(bar) : "memory");
   }
 
   // acc[row tile 2i and 2i + 1] += V words * B; f(i) gives the four words.
@@ -354,8 +367,8 @@ struct Kv8Attn {
     mma_f16(acc1, x0, x1, y0, y1, b0, b1);
   }
 
-  // Scores of the tile in kr; kr is free afterwards.
-  __device__ __forceinline__ void scores(const Smem& sm, float (&s)[NT][4], int lane) {
+  // Raw scores of a tile.
+  __device__ __forceinline__ void scores(const Smem& sm, uint32_t tile, float (&s)[NT][4], int lane) {
     float odd[NT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -363,8 +376,10 @@ struct Kv8Attn {
       for (int k = 0; k < 4; ++k) s[nt][k] = odd[nt][k] = 0.f;
 #pragma unroll
     for (int v = 0; v < kKVec; ++v) {
-      const uint32_t x[4] = {kr[0][v].x, kr[0][v].y, kr[0][v].z, kr[0][v].w};
-      const uint32_t y[4] = {kr[1][v].x, kr[1][v].y, kr[1][v].z, kr[1][v].w};
+      uint4 kr[2];
+      read_k(tile, v, lane, kr);
+      const uint32_t x[4] = {kr[0].x, kr[0].y, kr[0].z, kr[0].w};
+      const uint32_t y[4] = {kr[1].x, kr[1].y, kr[1].z, kr[1].w};
       uint32_t q[NT][4][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -398,7 +413,7 @@ struct Kv8Attn {
                                           bool edge, int lane) {
     const float tk = pow2i((int8_t)(exps & 0xff)), ev = (float)(int8_t)((exps >> 8) & 0xff);
     const float iv = pow2i(-(int8_t)((exps >> 8) & 0xff));
-    const int g = lane >> 2;
+    const int row = tile_row(lane >> 2);
     bool over = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -408,7 +423,7 @@ struct Kv8Attn {
       if (edge) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          if (tok + g + (k >> 1) * 8 >= sm.lim[nt * 8 + 2 * (lane & 3) + (k & 1)]) s[nt][k] = -INFINITY;
+          if (tok + row + (k >> 1) * 8 >= sm.lim[nt * 8 + 2 * (lane & 3) + (k & 1)]) s[nt][k] = -INFINITY;
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) over |= s[nt][k] > m[nt][k & 1] + 8.f;
@@ -452,10 +467,18 @@ struct Kv8Attn {
     }
   }
 
-  // O^T += V^T P^T of the tile in vr; vr is free afterwards.
-  __device__ __forceinline__ void product(const Smem& sm, int tok, const uint32_t (&p)[NT][2], const uint32_t (&rest)[NT][2],
-                                          bool edge, int lane) {
-    if (edge) not_finite(sm, tok, lane);
+  // O^T += V^T P^T of the tile in vr.
+  __device__ __forceinline__ void product(const Smem& sm, int tok, int len, const uint32_t (&p)[NT][2],
+                                          const uint32_t (&rest)[NT][2], bool edge, int lane) {
+    if (edge) {
+      // rows behind the sequence hold anything
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (tok + tile_row(2 * (lane & 3) + (r & 1)) + 8 * (r >> 1) >= len)
+#pragma unroll
+          for (int i = 0; i < kVWords; ++i) vr[r][i] = 0u;
+      not_finite(sm, tok, lane);
+    }
 #pragma unroll
     for (int i = 0; i < kVWords; ++i) {
       const uint32_t w[4] = {vr[0][i], vr[1][i], vr[2][i], vr[3][i]};
@@ -478,15 +501,15 @@ struct Kv8Attn {
 #pragma unroll
       for (int i = 0; i < kVWords; ++i) any |= nonfinite_bytes<E5M2>(vr[r][i]) != 0u;
     if (!__any_sync(0xffffffffu, any)) return;
-    const int g = lane >> 2;
+    const int row = tile_row(lane >> 2);
     constexpr uint32_t kOnes = E5M2 ? 0x3c3c3c3cu : 0x38383838u;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       uint32_t sees[2];
 #pragma unroll
       for (int k = 0; k < 2; ++k)
-        sees[k] = transpose8x8(pack_half2(tok + g + 8 * k < sm.lim[nt * 8 + 2 * (lane & 3)] ? 1.f : 0.f,
-                                          tok + g + 8 * k < sm.lim[nt * 8 + 2 * (lane & 3) + 1] ? 1.f : 0.f));
+        sees[k] = transpose8x8(pack_half2(tok + row + 8 * k < sm.lim[nt * 8 + 2 * (lane & 3)] ? 1.f : 0.f,
+                                          tok + row + 8 * k < sm.lim[nt * 8 + 2 * (lane & 3) + 1] ? 1.f : 0.f));
 #pragma unroll
       for (int i = 0; i < kVWords; ++i) {
         float n0[4] = {}, n1[4] = {};
@@ -509,7 +532,8 @@ struct Kv8Attn {
 
   // The CTA's tiles of the segment: the warp's share (every kWarps-th).  The first tile's codes are on their way
   // while the query is staged.
-  __device__ __forceinline__ void piece(const Kv8AttnDev& a, Smem& sm, const Place& at, int warp, int lane) {
+  __device__ __forceinline__ void piece(const Kv8AttnDev& a, const CUtensorMap* k_map, const CUtensorMap* v_map, Smem& sm, const Place& at,
+                                        uint32_t& turn, int warp, int lane) {
     const int b = at.b, h = at.h, rt = at.rt;
     const int first = (int)(at.at - at.start), last = (int)min(at.n, at.end - at.start);
     const int len = at.len;
@@ -520,12 +544,18 @@ struct Kv8Attn {
     // lane j describes this warp's tile 32*k + j; the next 32 are looked up halfway through
     Tile now{-1, 0, 0}, next{-1, 0, 0};
     if (lane < n) now = find(a, b, h, len, mine + lane * kWarps);
-    int page = __shfl_sync(0xffffffffu, now.page, 0), tok = __shfl_sync(0xffffffffu, now.tok, 0);
-    load_k(a, page, tok, h, len, lane);
-    load_v(a, page, tok, h, len, lane);
+    const uint32_t ring = smem_addr(&sm.ring[warp][0][0]), bars = smem_addr(&sm.arrived[warp][0]);
+    int stage = (int)(turn % kStages);            // of tile i; tile number turn + i of the warp
+#pragma unroll 1
+    for (int i = 0; i < kStages; ++i) {
+      const int page = __shfl_sync(0xffffffffu, now.page, i), tok = __shfl_sync(0xffffffffu, now.tok, i);
+      const int to = stage + i < kStages ? stage + i : stage + i - kStages;
+      if (lane == 0 && i < n) fetch(a, k_map, v_map, page, tok, h, ring + to * kTileBytes, bars + 8 * to);
+    }
     stage_q(a, sm, q, rt, len, warp, lane);
     __syncthreads();
     start(sm, lane);
+    uint32_t phase = (turn / kStages) & 1;
 #pragma unroll 1
     for (int i = 0; i < n; ++i) {
       if ((i & 31) == 16) {
@@ -533,24 +563,35 @@ struct Kv8Attn {
         next = Tile{-1, 0, 0};
         if (j < n) next = find(a, at.b, h, len, (int)(at.at - at.start) + warp + j * kWarps);
       }
-      const int exps = __shfl_sync(0xffffffffu, now.exps, i & 31);
-      if ((i & 31) == 31) now = next;
-      int page_ahead = __shfl_sync(0xffffffffu, now.page, (i + 1) & 31);
-      const int tok_ahead = __shfl_sync(0xffffffffu, now.tok, (i + 1) & 31);
-      if (i + 1 >= n) page_ahead = -1;
-      const bool edge = tok + 16 > seen_by_all;
-      float s[NT][4];
-      uint32_t p[NT][2], rest[NT][2];
-      if (page >= 0) scores(sm, s, lane);
-      load_k(a, page_ahead, tok_ahead, h, len, lane);
-      if (page >= 0) {
-        weights(sm, tok, exps, s, p, rest, edge, lane);
-        product(sm, tok, p, rest, edge, lane);
+      const int tok = __shfl_sync(0xffffffffu, now.tok, i & 31), exps = __shfl_sync(0xffffffffu, now.exps, i & 31);
+      const uint32_t tile = ring + stage * kTileBytes;
+      if (!__all_sync(0xffffffffu, bulk_wait(bars + 8 * stage, phase))) {
+        // never seen: the row would be wrong, so say so; the copies still in flight end before the CTA does
+        if (lane == 0 && a.status) atomicOr(a.status, MSKV_STATUS_TIMEOUT);
+        for (int k = 0; k < kStages; ++k) bulk_wait(bars + 8 * k, phase);
+        break;
       }
-      load_v(a, page_ahead, tok_ahead, h, len, lane);
-      page = page_ahead;
-      tok = tok_ahead;
+      if (exps & 0x10000) {
+        const bool edge = tok + 16 > seen_by_all;
+        float s[NT][4];
+        uint32_t p[NT][2], rest[NT][2];
+        scores(sm, tile, s, lane);
+        read_v(tile, lane);
+        weights(sm, tok, exps, s, p, rest, edge, lane);
+        product(sm, tok, len, p, rest, edge, lane);
+      }
+      // the tile kStages further takes the stage
+      const bool other = (i & 31) + kStages > 31;
+      const int page_ahead = __shfl_sync(0xffffffffu, other ? next.page : now.page, (i + kStages) & 31);
+      const int tok_ahead = __shfl_sync(0xffffffffu, other ? next.tok : now.tok, (i + kStages) & 31);
+      if (lane == 0 && i + kStages < n) fetch(a, k_map, v_map, page_ahead, tok_ahead, h, tile, bars + 8 * stage);
+      if (++stage == kStages) {
+        stage = 0;
+        phase ^= 1;
+      }
+      if ((i & 31) == 31) now = next;
     }
+    turn += n;
     collect(sm, warp, lane);
   }
 
@@ -776,13 +817,18 @@ __device__ __forceinline__ bool line_place(const Kv8AttnDev& a, Place& at, int l
 }
 
 template <int D, int NT, bool E5M2, bool BF16>
-__global__ void __launch_bounds__(32 * ka_warps(D, NT), ka_ctas(D, NT)) kv8_attn_kernel(const Kv8AttnDev a) {
+__global__ void __launch_bounds__(32 * ka_warps(D, NT), ka_ctas(D, NT))
+kv8_attn_kernel(const Kv8AttnDev a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
   using K = Kv8Attn<D, NT, E5M2, BF16>;
-  extern __shared__ __align__(16) char smem_raw[];
-  typename K::Smem& sm = *reinterpret_cast<typename K::Smem*>(smem_raw);
+  extern __shared__ uint8_t smem_raw[];
+  typename K::Smem& sm = *reinterpret_cast<typename K::Smem*>(smem_raw + (-smem_addr(smem_raw) & 1023u));
   __shared__ bool s_some;
   __shared__ Place at;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane == 0) {
+    for (int i = 0; i < K::kStages; ++i) mbar_init(smem_addr(&sm.arrived[warp][i]), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
   wait_for_previous_grid();
   allow_dependents();              // what follows may be set up from here on; it waits for this grid's end
   // The CTA's place is kept in shared memory: it would cost the tile loop registers.
@@ -810,8 +856,9 @@ __global__ void __launch_bounds__(32 * ka_warps(D, NT), ka_ctas(D, NT)) kv8_attn
   __syncthreads();
   if (!a.cluster && !s_some) return;
   K k;
+  uint32_t turn = 0;               // tiles that this warp has taken
   for (;;) {
-    k.piece(a, sm, at, warp, lane);
+    k.piece(a, &k_map, &v_map, sm, at, turn, warp, lane);
     if (a.cluster > 1) {
       K::finish_cluster(a, sm, at, blockIdx.x % a.cluster, a.cluster);
       return;
@@ -821,6 +868,7 @@ __global__ void __launch_bounds__(32 * ka_warps(D, NT), ka_ctas(D, NT)) kv8_attn
     K::finish(a, sm, at, cut ? 2 * (int)blockIdx.x + (at.at == at.begin ? 0 : 1) : -1);
     if (a.cluster) return;
     const bool done = at.start + last >= at.end;
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the warps' sums were ordinary stores to the ring's place
     __syncthreads();                                  // the buffers and the place have been read
     if (threadIdx.x == 0) {
       if (first == 0)
@@ -970,11 +1018,30 @@ static Kv8Plan make_plan(const mskv_kv8_attn_desc& d) {
   return p;
 }
 
+// K or V as a 4-D tensor [page][head][row][dim] of bytes, in boxes of 16 rows and at most 128 dims.
+static bool encode_pages_map(CUtensorMap* m, uint8_t* base, const Kv8Dev& pg, int d) {
+  const EncodeTiledFn encode = tensor_map_encoder();
+  if (!encode) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)pg.page_size, (cuuint64_t)pg.heads, (cuuint64_t)pg.num_pages};
+  // a single head or page has no stride of its own
+  const cuuint64_t page_bytes = (cuuint64_t)pg.page_size * d;
+  const cuuint64_t strides[3] = {(cuuint64_t)d, pg.heads > 1 ? (cuuint64_t)pg.sh : page_bytes,
+                                 pg.num_pages > 1 ? (cuuint64_t)pg.sp : page_bytes};
+  const cuuint32_t box[4] = {(cuuint32_t)std::min(d, 128), 16, 1, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  return encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                d < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int D, int NT, bool E5M2, bool BF16>
 static int launch_attn(const Kv8AttnDev& a, const Kv8Plan& p, cudaStream_t st) {
-  constexpr int smem = (int)sizeof(typename Kv8Attn<D, NT, E5M2, BF16>::Smem);
+  constexpr int smem = (int)sizeof(typename Kv8Attn<D, NT, E5M2, BF16>::Smem) + 1024;   // + the ring's alignment
   const auto kernel = kv8_attn_kernel<D, NT, E5M2, BF16>;
   if (const int rc = ensure_smem_limit(reinterpret_cast<const void*>(kernel), smem, "mskv_kv8_attention")) return rc;
+  CUtensorMap maps[2];
+  if (!encode_pages_map(&maps[0], a.pg.k, a.pg, D) || !encode_pages_map(&maps[1], a.pg.v, a.pg, D))
+    return fail(MSKV_ERR_CUDA, "mskv_kv8_attention: the cache's layout cannot be encoded for TMA");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)p.ctas);
   cfg.blockDim = dim3(32 * ka_warps(D, NT));
@@ -988,7 +1055,7 @@ static int launch_attn(const Kv8AttnDev& a, const Kv8Plan& p, cudaStream_t st) {
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = p.cluster > 1 ? 2 : 1;
-  const cudaError_t launched = cudaLaunchKernelEx(&cfg, kernel, a);
+  const cudaError_t launched = cudaLaunchKernelEx(&cfg, kernel, a, maps[0], maps[1]);
   if (launched != cudaSuccess) return cuda_status(launched, "mskv_kv8_attention launch");
   if (const int rc = after_launch("mskv_kv8_attention")) return rc;
   if (p.cluster) return MSKV_OK;
@@ -1015,6 +1082,11 @@ static int check_attn(const mskv_kv8_attn_desc* d) {
   if (!d) return fail(MSKV_ERR_ARG, "%s: NULL descriptor", what);
   if (const int rc = check_kv8(d->pages, what)) return rc;
   if (d->dtype != MSKV_DT_BF16 && d->dtype != MSKV_DT_F16) return fail(MSKV_ERR_DTYPE, "%s: q and out must be bf16 or f16", what);
+  constexpr int64_t kMaxStride = (int64_t)1 << 40;
+  if ((d->pages.kv_heads > 1 && (d->pages.stride_h <= 0 || d->pages.stride_h >= kMaxStride)) ||
+      (d->pages.num_pages > 1 && (d->pages.stride_page <= 0 || d->pages.stride_page >= kMaxStride)) ||
+      d->pages.num_pages > INT_MAX)
+    return fail(MSKV_ERR_RANGE, "%s: stride_page and stride_h must lie in (0, 2^40), num_pages below 2^31", what);
   if (d->q_heads <= 0 || d->q_heads % d->pages.kv_heads)
     return fail(MSKV_ERR_ARG, "%s: q_heads must be a multiple of kv_heads", what);
   if (d->q_len <= 0 || d->q_len > MSKV_KV8_MAX_QLEN)
