@@ -540,10 +540,10 @@ struct Kv8Attn {
     const int seen_by_all = len - a.q_len + 1;    // tokens below: every row sees them
     const int mine = first + warp;
     const int n = mine < last ? (last - mine + kWarps - 1) / kWarps : 0;
-    const QRows q = load_q(a, b, h, rt, warp, lane);
     // lane j describes this warp's tile 32*k + j; the next 32 are looked up halfway through
     Tile now{-1, 0, 0}, next{-1, 0, 0};
     if (lane < n) now = find(a, b, h, len, mine + lane * kWarps);
+    const QRows q = load_q(a, b, h, rt, warp, lane);
     const uint32_t ring = smem_addr(&sm.ring[warp][0][0]), bars = smem_addr(&sm.arrived[warp][0]);
     int stage = (int)(turn % kStages);            // of tile i; tile number turn + i of the warp
 #pragma unroll 1
@@ -825,6 +825,10 @@ kv8_attn_kernel(const Kv8AttnDev a, const __grid_constant__ CUtensorMap k_map, c
   __shared__ bool s_some;
   __shared__ Place at;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
+  }
   if (lane == 0) {
     for (int i = 0; i < K::kStages; ++i) mbar_init(smem_addr(&sm.arrived[warp][i]), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -1006,11 +1010,13 @@ static Kv8Plan make_plan(const mskv_kv8_attn_desc& d) {
     p.ctas = p.segments * cluster;
     return p;
   }
-  p.ctas = std::min<int64_t>(slots, (p.segments * most + warps - 1) / warps);
-  // Parts that do not cross segments leave CTAs without work (at 128 segments 256 of 296 have some), a part
-  // that does costs a second start.  28/4 heads, 8 sequences of 16384 tokens (111 tiles a CTA): 33.0 us
-  // against 37.1; 40/8 heads, 16 of 32768 (886 a CTA): 199 us against 185.
-  p.aligned = p.segments * 2 <= p.ctas && p.segments * most <= 256 * p.ctas;
+  // Long lines in twice as many parts, so that CTAs which get less of the memory's bandwidth take fewer: 40/8
+  // heads, 16 sequences of 32768 tokens (886 tiles a CTA in one wave) 174 us against 181; 28/4 heads, 8 of
+  // 16384 (111 a CTA) 36.8 against 32.2, as the second wave starts its pipelines anew.
+  p.ctas = std::min<int64_t>(p.segments * most > 512 * slots ? 2 * slots : slots, (p.segments * most + warps - 1) / warps);
+  // Parts that do not cross segments leave some CTAs without work, a part that does costs a second start:
+  // 33.0 us against 37.1 for the 8 sequences of 16384 tokens above.
+  p.aligned = p.segments * 2 <= p.ctas;
   const uint64_t rows_held = 2 * (uint64_t)p.ctas * p.nt * 8;
   p.info_bytes = ((uint64_t)p.segments * sizeof(int4) + 255) / 256 * 256;
   p.ml_bytes = (rows_held * 2 * sizeof(float) + 255) / 256 * 256;
