@@ -1,0 +1,153 @@
+"""An HBM-resident KV cache in 8 bits for a fixed batch of sequences.
+
+Beside the offload engine (engine.OffloadKV: 16-bit KV in host memory, selected rows over the host link)
+for sequences that fit HBM at one byte per value: K and V of every layer in 8-bit pages with a
+power-of-two scale per (page, KV head) and the pages' key bounds (ops.Kv8Pages), one int32 page table
+[B, max_pages] shared by all layers.  No counterpart in the reference.
+
+A decode step, per layer: the step's tokens are appended (mskv_kv8_append), then either the whole cache is
+attended (mskv_kv8_attention) or, with ``top_blocks``, every page is scored from its bounds
+(mskv_kv8_block_score), the best pages and the last ``recent_blocks`` are selected per (sequence, KV head)
+(mskv_topk) and attention runs over those.  No host synchronisation: ``begin_step`` sends the step's
+lengths through pinned staging, so the per-layer calls can be captured once in a CUDA graph and replayed
+while the cache grows.
+"""
+from __future__ import annotations
+
+from typing import List, Optional, Sequence, Union
+
+import numpy as np
+import torch
+
+from . import ops
+
+
+class PagedKV8:
+    """8-bit paged KV of num_layers layers for `batch` sequences of up to `capacity` tokens.
+
+    q_heads, kv_heads, head_dim: the model's (this rank's share, when heads are sharded); page_size: tokens
+    per page; cache_dtype: torch.float8_e4m3fn or torch.float8_e5m2.  top_blocks > 0: attention over the
+    top_blocks best pages and the last recent_blocks (at least 1: the step's own tokens) of
+    every (sequence, KV head); 0: over the whole cache.
+    """
+
+    def __init__(self, num_layers: int, batch: int, q_heads: int, kv_heads: int, head_dim: int, capacity: int, *,
+                 top_blocks: int = 0, recent_blocks: int = 1, page_size: int = 16,
+                 cache_dtype: torch.dtype = torch.float8_e4m3fn, device: Optional[torch.device] = None):
+        if batch <= 0 or kv_heads <= 0 or q_heads <= 0 or q_heads % kv_heads:
+            raise ValueError("q_heads must be a positive multiple of kv_heads, batch positive")
+        if capacity <= 0:
+            raise ValueError("capacity must be positive")
+        if top_blocks < 0 or (top_blocks > 0 and recent_blocks < 1):
+            raise ValueError("top_blocks must be >= 0, and recent_blocks >= 1 with it")
+        self.device = ops._norm(device if device is not None else "cuda")
+        self.L, self.B, self.Hq, self.Hkv, self.D = num_layers, batch, q_heads, kv_heads, head_dim
+        self.C, self.page_size = int(capacity), int(page_size)
+        self.top_blocks, self.recent_blocks = int(top_blocks), int(recent_blocks)
+        self.max_pages = (self.C + page_size - 1) // page_size
+        self.num_pages = batch * self.max_pages
+        self.pages: List[ops.Kv8Pages] = [
+            ops.kv8_pages(self.num_pages, kv_heads, head_dim, page_size=page_size, dtype=cache_dtype, device=self.device,
+                          bounds=top_blocks > 0)
+            for _ in range(num_layers)]
+        self._free = list(range(self.num_pages - 1, -1, -1))
+        self.page_table_h = np.full((batch, self.max_pages), -1, dtype=np.int32)
+        self.page_table = torch.full((batch, self.max_pages), -1, dtype=torch.int32, device=self.device)
+        self.len_h = np.zeros(batch, dtype=np.int64)
+        # the step's state on the device: lengths before it, tokens it appends, lengths and blocks after it
+        self._state = torch.zeros(4, batch, dtype=torch.int32, device=self.device)
+        self.tok0, self.n_new, self.lens, self.held = self._state.unbind(0)
+        self._stage = torch.zeros(4, batch, dtype=torch.int32).pin_memory()
+        self._pt_stage = torch.empty(batch, self.max_pages, dtype=torch.int32).pin_memory()
+        self._stage_ev: Optional[torch.cuda.Event] = None
+        if top_blocks:
+            self._scores = torch.empty(batch, kv_heads, self.max_pages, dtype=torch.float32, device=self.device)
+            self._idx = torch.empty(batch * kv_heads, top_blocks + recent_blocks, dtype=torch.int32, device=self.device)
+            self._counts = torch.empty(batch * kv_heads, dtype=torch.int32, device=self.device)
+
+    # ------------------------------------------------------------------ lengths and pages
+    def begin_step(self, n_new: Union[int, Sequence[int]] = 1) -> None:
+        """Room for n_new tokens of every sequence (an int, or one number each; 0 leaves a sequence as it is).
+
+        Maps the pages they need and sets the device-side lengths, through pinned staging copies on the current
+        stream (the host waits only for the previous step's).  append_layer then writes each layer's rows
+        and decode_layer attends over the grown cache.
+        """
+        n_new = np.broadcast_to(np.asarray(n_new, dtype=np.int64), (self.B,))
+        if (n_new < 0).any():
+            raise ValueError("n_new must not be negative")
+        new_len = self.len_h + n_new
+        if (new_len > self.C).any():
+            raise ValueError(f"a step exceeds the capacity of {self.C} tokens per sequence")
+        # a page for every position up to the new lengths: batch * max_pages of them exist, so one is always free
+        mapped = False
+        for b in range(self.B):
+            for p in range(int(self.len_h[b]) // self.page_size, -(-int(new_len[b]) // self.page_size)):
+                if self.page_table_h[b, p] < 0:
+                    self.page_table_h[b, p] = self._free.pop()
+                    mapped = True
+        self._send(self.len_h, n_new, new_len, mapped)
+        self.len_h = new_len
+
+    def reset(self, b: int) -> None:
+        """Empties sequence b: its pages are free for others from the next step on."""
+        if not 0 <= b < self.B:
+            raise ValueError(f"no sequence {b}")
+        row = self.page_table_h[b]
+        self._free.extend(int(p) for p in row[row >= 0])
+        row[:] = -1
+        self.len_h = self.len_h.copy()
+        self.len_h[b] = 0
+        self._send(self.len_h, np.zeros(self.B, dtype=np.int64), self.len_h, True)
+
+    def _send(self, old: np.ndarray, n_new: np.ndarray, new: np.ndarray, table: bool) -> None:
+        if self._stage_ev is not None:
+            self._stage_ev.synchronize()        # the staging buffers' last copies are done
+        st = self._stage.numpy()
+        st[0], st[1], st[2], st[3] = old, n_new, new, -(-new // self.page_size)
+        with torch.cuda.device(self.device):
+            if table:
+                self._pt_stage.numpy()[:] = self.page_table_h
+                self.page_table.copy_(self._pt_stage, non_blocking=True)
+            self._state.copy_(self._stage, non_blocking=True)
+            self._stage_ev = torch.cuda.Event()
+            self._stage_ev.record(torch.cuda.current_stream(self.device))
+
+    # ------------------------------------------------------------------ a layer of the step
+    def append_layer(self, layer: int, k_new: torch.Tensor, v_new: torch.Tensor) -> None:
+        """The step's rows [B, Hkv, n, D] of one layer (n at least every sequence's n_new; fp32, fp16 or bf16)."""
+        if k_new.dim() != 4 or k_new.shape[:2] != (self.B, self.Hkv) or k_new.shape[3] != self.D:
+            raise ValueError(f"k_new must be [B={self.B}, Hkv={self.Hkv}, n, D={self.D}]")
+        if k_new.shape[2] < int(self._stage[1].max()):
+            raise ValueError(f"the step appends up to {int(self._stage[1].max())} tokens, k_new holds {k_new.shape[2]}")
+        ops.kv8_append(self.pages[layer], self.page_table, k_new, v_new, tok0=self.tok0, counts=self.n_new)
+
+    def select(self, layer: int, q: torch.Tensor):
+        """Pages for q's last position: (indices [B, Hkv, top + recent], ascending, counts [B, Hkv])."""
+        ops.kv8_block_score(q, self.pages[layer], self.page_table, lens=self.lens, max_blocks=self.max_pages,
+                            out=self._scores)
+        ops.topk(self._scores.view(self.B * self.Hkv, self.max_pages), top_k=self.top_blocks, recent=self.recent_blocks,
+                 len_=self.held, len_scalar=self.max_pages, sel_per_batch=self.Hkv, out=self._idx, counts=self._counts)
+        return self._idx.view(self.B, self.Hkv, -1), self._counts.view(self.B, self.Hkv)
+
+    def decode_layer(self, layer: int, q: torch.Tensor, *, out: Optional[torch.Tensor] = None,
+                     t_bound: Optional[int] = None) -> torch.Tensor:
+        """Attention of the last Q tokens over one layer's cache: q [B, Hq, Q, D] (or [B, Hq, D]) -> [B, Hq, Q, D].
+
+        Position i of a sequence of length n sees the tokens below n - Q + 1 + i.  t_bound: the length bound
+        that the kernel is launched for (default: the capacity, which stays valid in a captured step while the
+        cache grows).
+        """
+        if q.dim() == 3:
+            q = q.unsqueeze(2)
+        if self.top_blocks:
+            idx, counts = self.select(layer, q)
+            return ops.kv8_attention(q, self.pages[layer], self.page_table, lens=self.lens, blocks=idx, counts=counts, out=out)
+        return ops.kv8_attention(q, self.pages[layer], self.page_table, lens=self.lens,
+                                 max_tokens=self.C if t_bound is None else t_bound, out=out)
+
+    def step_layer(self, layer: int, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, *,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """append_layer and decode_layer: one layer of a decode step."""
+        self.append_layer(layer, k_new, v_new)
+        return self.decode_layer(layer, q, out=out)
