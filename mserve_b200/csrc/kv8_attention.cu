@@ -1001,11 +1001,21 @@ static Kv8Plan make_plan(const mskv_kv8_attn_desc& d) {
   const int64_t most = d.blocks ? (int64_t)d.num_blocks * (d.pages.page_size / 16) : ((int64_t)d.max_tokens + 15) / 16;
   const int warps = ka_warps(d.pages.head_dim, p.nt);
   const int64_t slots = (int64_t)num_sms() * ka_ctas(d.pages.head_dim, p.nt);   // CTAs that run at once
-  // One cluster a segment, merged in its shared memory: while a warp has up to four tiles, and for lists, which
-  // are of one length as a rule, wherever the clusters fill most of the GPU.  Two tiles a warp decide its size.
-  int cluster = 1;
+  // A cluster of 1 to 8 CTAs for each segment, merged in its shared memory: no line to find one's place on, no
+  // second kernel, but the segments wait for the longest.  Chosen
+  //  * for short segments (up to four tiles a warp), with two tiles a warp or less;
+  //  * where the clusters fill four fifths of the GPU or more and all of it at most (at two thirds, 32/8 heads of 64
+  //    dims, 4 positions, 6 ragged sequences: 26.5 us against 19.4): for lists, which are of one
+  //    length as a rule, and for up to 32 tiles a warp: 28/4 heads, 8 sequences of 16384 tokens 28.1 us against
+  //    32.4 on the line, 16 of 4096 17.7 against 20.8, 64 of up to 4096 41.2 against 46.1; ragged down to an
+  //    eighth, 8 of up to 16384: 23.5 against 22.7.  Longer ones not: 40/8 heads, 16 of 32768, ragged: 144 us in
+  //    clusters of two, 107 on the line (equal lengths: 175 and 173).
+  int cluster = 1, fill = 1;
   while (cluster < kKaMaxCluster && most > 2 * warps * cluster && p.segments * cluster * 2 <= slots) cluster *= 2;
-  if (most <= 4 * warps * cluster || (d.blocks && p.segments <= slots && p.segments * cluster * 5 >= slots * 3)) {
+  while (fill < kKaMaxCluster && p.segments * fill * 2 <= slots) fill *= 2;
+  const bool fills = p.segments * fill <= slots && p.segments * fill * 5 >= slots * 4;
+  if (most > 4 * warps * cluster && fills && (d.blocks || most <= 32 * warps * fill)) cluster = fill;
+  if (most <= 4 * warps * cluster || (fills && cluster == fill && (d.blocks || most <= 32 * warps * fill))) {
     p.cluster = cluster;
     p.ctas = p.segments * cluster;
     return p;
