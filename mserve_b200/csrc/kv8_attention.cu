@@ -144,6 +144,8 @@ struct Kv8Attn {
       uint8_t ring[kWarps][kStages][kTileBytes];  // 1024-byte aligned stages (the swizzle's period)
       float o[kWarps][kRows][kOStride];           // the warps' sums, when the ring is empty; o[0], m[0], l[0] then the CTA's
     };
+    float sent[kRows][D];                         // of the cluster's CTAs: [CTA][rows of this one]
+    float2 sent_ml[kRows];
     uint64_t arrived[kWarps][kStages];            // mbarriers
     float m[kWarps][kRows], l[kWarps][kRows];
     __half q[kRows][D + 8];
@@ -666,62 +668,40 @@ struct Kv8Attn {
     }
   }
 
-  // The same for a cluster of `ctas` CTAs that share a segment: every CTA sums its warps in place, then finishes the
-  // rows of its rank from all the CTAs' shared memory.
+  // The same for a cluster of `ctas` CTAs that share a segment: every CTA stores its sums of row r into the shared
+  // memory of CTA r % ctas, which finishes the row after one barrier of the cluster (nothing reads another
+  // CTA's memory after that, so each may end).
   static __device__ __forceinline__ void finish_cluster(const Kv8AttnDev& a, Smem& sm, const Place& at, int rank, int ctas) {
-    constexpr int kEach = (kRows * D / 4 + kThreads - 1) / kThreads;
-    Part y[kEach];
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      const int i = threadIdx.x + e * kThreads;
-      if (i < kRows * D / 4) y[e] = cta_part(sm, i / (D / 4), (i % (D / 4)) * 4);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      const int i = threadIdx.x + e * kThreads, r = i / (D / 4), d = (i % (D / 4)) * 4;
-      if (i < kRows * D / 4) {
-        *reinterpret_cast<float4*>(&sm.o[0][r][d]) = y[e].x;
-        if (d == 0) {
-          sm.m[0][r] = y[e].top;
-          sm.l[0][r] = y[e].sum;
-        }
-      }
-    }
     cg::cluster_group cluster = cg::this_cluster();
+    cluster.barrier_wait();                       // all CTAs of the cluster run (they arrived when they began)
+#pragma unroll 1
+    for (int i = threadIdx.x; i < kRows * D / 4; i += kThreads) {
+      const int r = i / (D / 4), d = (i % (D / 4)) * 4, owner = r % ctas, slot = rank * ((kRows + ctas - 1) / ctas) + r / ctas;
+      const Part y = cta_part(sm, r, d);
+      *cluster.map_shared_rank(reinterpret_cast<float4*>(&sm.sent[slot][d]), owner) = y.x;
+      if (d == 0) *cluster.map_shared_rank(&sm.sent_ml[slot], owner) = make_float2(y.top, y.sum);
+    }
     cluster.sync();
-    // a row is a stretch of D/4 threads; ranks take rows in turn
+    const int each = (kRows + ctas - 1) / ctas;   // rows of a CTA; a row is a stretch of D/4 threads
     const int stretch = threadIdx.x / (D / 4), d = (threadIdx.x % (D / 4)) * 4;
 #pragma unroll 1
-    for (int r = rank + stretch * ctas; r < kRows; r += kThreads / (D / 4) * ctas) {
+    for (int k = stretch; k < each; k += kThreads / (D / 4)) {
+      const int r = k * ctas + rank;
       if (at.rt * kRows + r >= a.rows) break;
       float top = kNoMax, sum = 0.f;
+#pragma unroll 1
+      for (int c = 0; c < ctas; ++c) top = fmaxf(top, sm.sent_ml[c * each + k].x);
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-      // all remote loads at once: one round trip
-      float m[kKaMaxCluster], l[kKaMaxCluster];
-      float4 z[kKaMaxCluster];
-#pragma unroll
-      for (int c = 0; c < kKaMaxCluster; ++c) {
-        m[c] = kNoMax;
-        l[c] = 0.f;
-        z[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (c < ctas) {
-          m[c] = *cluster.map_shared_rank(&sm.m[0][r], c);
-          l[c] = *cluster.map_shared_rank(&sm.l[0][r], c);
-          z[c] = *cluster.map_shared_rank(reinterpret_cast<float4*>(&sm.o[0][r][d]), c);
-        }
-      }
-#pragma unroll
-      for (int c = 0; c < kKaMaxCluster; ++c) top = fmaxf(top, m[c]);
-#pragma unroll
-      for (int c = 0; c < kKaMaxCluster; ++c) {
-        const float is = exp2_fast(m[c] - top);
-        x.x += z[c].x * is; x.y += z[c].y * is; x.z += z[c].z * is; x.w += z[c].w * is;
-        sum += l[c] * is;
+#pragma unroll 2
+      for (int c = 0; c < ctas; ++c) {
+        const float2 ml = sm.sent_ml[c * each + k];
+        const float is = exp2_fast(ml.x - top);
+        const float4 z = *reinterpret_cast<const float4*>(&sm.sent[c * each + k][d]);
+        x.x += z.x * is; x.y += z.y * is; x.z += z.z * is; x.w += z.w * is;
+        sum += ml.y * is;
       }
       write_out(a, at.b, at.h, at.rt * kRows + r, d, x, sum);
     }
-    cluster.sync();                               // the others may still read this CTA's sums
   }
 
   // out[row][d .. d+3] = x / sum, 0 for a row that saw nothing.
@@ -829,6 +809,7 @@ kv8_attn_kernel(const Kv8AttnDev a, const __grid_constant__ CUtensorMap k_map, c
     asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
   }
+  if (a.cluster > 1) cg::this_cluster().barrier_arrive();
   if (lane == 0) {
     for (int i = 0; i < K::kStages; ++i) mbar_init(smem_addr(&sm.arrived[warp][i]), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");

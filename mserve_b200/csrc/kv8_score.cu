@@ -41,19 +41,18 @@ __global__ void __launch_bounds__(kBsWarps * 32, D <= 128 ? 4 : 2) kv8_block_sco
   allow_dependents();
   const int bh = blockIdx.x / a.chunks, chunk = blockIdx.x - bh * a.chunks;
   const int b = bh / a.pg.heads, h = bh - b * a.pg.heads;
-  const int64_t len = min((int64_t)max(a.lens[b], 0), (int64_t)a.max_blocks * a.pg.page_size);
-  const int held = (int)((len + a.pg.page_size - 1) / a.pg.page_size);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int first = chunk * a.tiles * kBsWarps * 16;
+  const int j0 = first + warp * 16 + g;
+  const int32_t* const table = a.pg.page_table + (int64_t)b * a.pg.pt_stride;
+  // the first tile's table entries, before the length is known
+  const int entry[2] = {j0 < a.max_blocks ? table[j0] : -1, j0 + 8 < a.max_blocks ? table[j0 + 8] : -1};
+  const int64_t len = min((int64_t)max(a.lens[b], 0), (int64_t)a.max_blocks * a.pg.page_size);
+  const int held = (int)(((uint32_t)len + a.pg.page_size - 1) / a.pg.page_size);
   if (first >= held) return;                // the whole CTA
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  const int32_t* const table = a.pg.page_table + (int64_t)b * a.pg.pt_stride;
   // Block j's page: -2 where there is no block, -1 where its page is unmapped.
-  const auto page_of = [&](int j) {
-    if (j >= held) return -2;
-    const int p = table[j];
-    return p >= 0 && p < a.pg.num_pages ? p : -1;
-  };
+  const auto page_of = [&](int j, int p) { return j >= held ? -2 : p >= 0 && p < a.pg.num_pages ? p : -1; };
   uint4 x[2][kVec];
   int e[2];
   const auto load = [&](const int (&page)[2]) {
@@ -72,8 +71,7 @@ __global__ void __launch_bounds__(kBsWarps * 32, D <= 128 ? 4 : 2) kv8_block_sco
     }
   };
   // the first tile's bounds are on their way while the weights are made
-  const int j0 = first + warp * 16 + g;
-  int page[2] = {page_of(j0), page_of(j0 + 8)};
+  int page[2] = {page_of(j0, entry[0]), page_of(j0 + 8, entry[1])};
   load(page);
 
   // weights: sums over the heads, then both terms at a common power of two
@@ -122,8 +120,11 @@ __global__ void __launch_bounds__(kBsWarps * 32, D <= 128 ? 4 : 2) kv8_block_sco
     if (j - g >= held) break;
     int ahead[2] = {-2, -2};
     if (t + 1 < a.tiles) {
-      ahead[0] = page_of(j + kBsWarps * 16);
-      ahead[1] = page_of(j + kBsWarps * 16 + 8);
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int k = j + kBsWarps * 16 + 8 * r;
+        ahead[r] = page_of(k, k < held ? table[k] : -1);
+      }
     }
     float acc[2][4] = {};                   // two chains of k-steps
 #pragma unroll
