@@ -51,6 +51,16 @@ inline int check_kv8(const mskv_kv8_pages& p, const char* what) {
   return MSKV_OK;
 }
 
+// Multiprocessors of the current device, asked for once per device (two plans a call).
+inline int sms_of_device() {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return num_sms();
+  int n = known[dev].load(std::memory_order_relaxed);
+  if (n == 0) known[dev].store(n = num_sms(), std::memory_order_relaxed);
+  return n;
+}
+
 // 2^e for e in [-126, 127].
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 

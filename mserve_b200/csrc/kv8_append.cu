@@ -415,7 +415,7 @@ extern "C" int mskv_kv8_append(const mskv_kv8_append_desc* d, void* stream) {
   a.all_units = (uint32_t)all;
   // Units of 2 * page_size/16 warps: up to 8 warps a CTA, but one unit each while every SM has room for them
   // (a decode token of 8 sequences, 4 heads: 2.7 us against 3.3).
-  const bool few = all <= 4 * (int64_t)num_sms();
+  const bool few = all <= 4 * (int64_t)sms_of_device();
   a.units = few ? 1 : (uint32_t)std::max(1, 64 / a.pg.page_size);
   const int64_t ctas = (all + a.units - 1) / a.units;
   if (all > INT_MAX) return fail(MSKV_ERR_RANGE, "mskv_kv8_append: too many rows for one call");

@@ -893,10 +893,11 @@ __global__ void __launch_bounds__(kKmWarps * 32) kv8_merge_kernel(const Kv8AttnD
   const int rt = seg % a.row_tiles, bh = seg / a.row_tiles;
   const int b = bh / a.pg.heads, h = bh % a.pg.heads;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the lengths are those that the first kernel, which waited for whatever wrote them, has read already
+  const bool empty = kv8_tiles(a, b, h) == 0;
   wait_for_previous_grid();
   allow_dependents();
   if (rt * kRows + r >= a.rows) return;
-  const bool empty = kv8_tiles(a, b, h) == 0;
   float top = kNoMax, sum = 0.f;
   float x[kPer] = {};
   if (!empty) {
@@ -981,7 +982,7 @@ static Kv8Plan make_plan(const mskv_kv8_attn_desc& d) {
   p.segments = (int64_t)d.pages.batch * d.pages.kv_heads * p.row_tiles;
   const int64_t most = d.blocks ? (int64_t)d.num_blocks * (d.pages.page_size / 16) : ((int64_t)d.max_tokens + 15) / 16;
   const int warps = ka_warps(d.pages.head_dim, p.nt);
-  const int64_t slots = (int64_t)num_sms() * ka_ctas(d.pages.head_dim, p.nt);   // CTAs that run at once
+  const int64_t slots = (int64_t)sms_of_device() * ka_ctas(d.pages.head_dim, p.nt);   // CTAs that run at once
   // A cluster of 1 to 8 CTAs for each segment, merged in its shared memory: no line to find one's place on, no
   // second kernel, but the segments wait for the longest.  Chosen
   //  * for short segments (up to four tiles a warp), with two tiles a warp or less;

@@ -205,7 +205,7 @@ extern "C" int mskv_kv8_block_score(const mskv_kv8_score_desc* d, void* stream) 
   // weights' set-up is shared.
   const int64_t segs = (int64_t)a.pg.batch * a.pg.heads;
   const int64_t rows = ((int64_t)d->max_blocks + 16 * kBsWarps - 1) / (16 * kBsWarps);
-  a.tiles = (int)std::min<int64_t>(4, std::max<int64_t>(1, segs * rows / (2 * num_sms())));
+  a.tiles = (int)std::min<int64_t>(4, std::max<int64_t>(1, segs * rows / (2 * sms_of_device())));
   a.chunks = (int)((rows + a.tiles - 1) / a.tiles);
   const int64_t ctas = segs * a.chunks;
   if (ctas > INT_MAX) return fail(MSKV_ERR_RANGE, "mskv_kv8_block_score: too many blocks for one call");
