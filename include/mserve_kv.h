@@ -456,6 +456,8 @@ int mskv_kv8_block_score(const mskv_kv8_score_desc* d, void* stream);
  * sums in fp32; softmax weights enter the second product as fp16 (two fp16 terms for fp16
  * outputs).  `workspace` must hold mskv_kv8_attention_workspace_bytes(d) bytes of device memory,
  * 16-byte aligned; every launch writes all it reads of it.  Calls that may overlap must not share one.
+ * stride_page and stride_h must lie in (0, 2^40) here (codes are loaded by TMA).  Every wait on such a load
+ * is bounded; one that runs out leaves the row incomplete and sets MSKV_STATUS_TIMEOUT.
  * q (b, hq, i, d) at q + b*q_stride_b + hq*q_stride_h + i*q_stride_q (bytes) + d elements, out
  * likewise.                                                                                 */
 typedef struct mskv_kv8_attn_desc {

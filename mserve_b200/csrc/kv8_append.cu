@@ -9,12 +9,13 @@
 // A unit is a (page, KV head): page_size/16 warps for K and as many for V, each with 16 rows of its half, 8
 // neighbouring elements of a row per lane and step; a CTA of 8 warps has as many units as fit (one unit
 // of 2 warps a CTA: 16400 CTAs for 2 x 16384 tokens of 8 heads start no faster than 77 us).
-//  * Pages that only receive 16-bit rows (a prompt's) hold them as loaded, packed: every row is
-//    read once; the maximum is an integer maximum over the packed magnitudes, and the
-//    bounds are packed minima and maxima of the inputs, as rounding keeps their order.
-//  * Other pages (a decode token joins old rows; fp32 rows) read their rows twice, the second time
-//    from the caches: first for the maximum and the bounds, then for the codes.  Old rows are
-//    stored again only when the exponent changed.
+//  * A page that only receives 16-bit rows (a prompt's) holds them as loaded, packed: every row is read
+//    once; the maximum and the bounds are packed too (the bounds of the inputs, as rounding keeps their order).
+//  * Other pages (a decode token joins old rows; fp32 rows) take their rows as fp32, a batch of steps at a time,
+//    a second time from the caches where one batch does not hold them.  Old rows are stored again only
+//    when the exponent changed.
+// Measured: 2 x 16384 bf16 tokens, 8 heads, 128 dims (206 MB) 39 us = 0.80 of the copy rate; 4 x up to 64 fp16 tokens,
+// 8 heads 4.3 us; one token of 8 sequences, 4 heads 3.0 us (launch, length, page id, rows).
 #include <algorithm>
 #include <type_traits>
 

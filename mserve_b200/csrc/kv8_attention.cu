@@ -18,20 +18,27 @@
 // own rounding.  All sums are fp32.
 //
 // Bound by the codes' bytes (2D a token and KV head).  mma.sync m16n8k16 with the tokens on M:
-// S^T = K Q^T, O^T = V^T P^T, so the 8 columns hold the query rows (16 rows: two column tiles).
-// A warp owns a tile.  The contraction's order is free, so a lane's 16 contiguous codes of a K row are four
-// k-steps', and those of four V rows are eight row tiles' (byte permutations pair the tokens): 16-byte loads
-// straight from global memory into the fragments' registers, no shared memory and no barrier on the way; K of
-// the next tile is in flight during the softmax, V during the next scores.  (The same chunks through
-// cp.async into a ring of three tiles a warp: 257 us instead of 185 for 16 x 32768 tokens of 8 heads.)
-// A tcgen05 MMA would need 64 or 128 rows of f16 operands staged in shared memory after a
-// conversion there; the legacy pipe is a fifth busy at the memory's speed.
+// S^T = K Q^T, O^T = V^T P^T, so the 8 columns hold the query rows (16 rows: two column tiles, and
+// the codes converted once for both).
+// A warp owns a tile and a ring of tiles in flight: one lane starts a TMA box of 16 rows of K and one of V,
+// completing on the stage's mbarrier, three to six tiles ahead; nothing in the loop waits for another warp.
+// The contraction's order is free, so the 16 contiguous codes that a lane reads of a K row are four
+// k-steps', and those of four V rows are eight row tiles' (byte permutations pair the tokens); TMA's
+// swizzle keeps these 16-byte reads free of bank conflicts.
+// A tcgen05 MMA would need 64 or 128 rows of f16 operands staged in shared memory after a conversion there;
+// the legacy pipe is a fifth busy at the memory's speed.
 //
-// Split: all tiles of all (sequence, KV head, row tile) segments form one line, cut into parts
-// for the CTAs however ragged the lengths are (a scan over the lengths in every warp).  The 8 warps of a
-// CTA take a segment's tiles in turn and merge in shared memory; a segment of several CTAs goes
-// through the workspace and a second kernel.  Segments of few tiles go to one CTA or cluster
-// each and need neither.
+// Split: a segment is a (sequence, KV head, row tile).  Where the segments fill the GPU evenly, or are short, a
+// thread-block cluster takes each and merges through distributed shared memory.  Otherwise all tiles of all
+// segments form one line, cut into parts for the CTAs however ragged the lengths are (a scan over the
+// lengths in every CTA); a segment of several parts goes through the workspace and a second kernel.
+//
+// Measured (device time, three sets of inputs in turn): 40/8 heads, 128 dims, 16 sequences of 32768 tokens
+// (1.07 GB) 173 us = 0.95 of the copy rate; 28/4 heads, 8 of 16384 (134 MB) 28.3 us = 0.73, of which 4.5 us pass
+// before the first codes are there and 3 after the last; 136 listed pages of each (18 MB) 9.3 us.
+// Loads straight into registers instead of the ring (one tile ahead, as many as the registers hold): 181,
+// 32.5 and 11.7 us, and 10% more than that at the clocks of a GPU at its power limit; the same chunks through
+// cp.async into a ring: 257 us for the first.
 #include <cooperative_groups.h>
 #include <math.h>
 
@@ -63,13 +70,13 @@ struct Kv8AttnDev {
   int32_t vec_q, pow2_page, aligned;
 };
 
-// Warps of a CTA and CTAs of an SM, by what the registers hold: at 64 and 128 dims, up to 8 rows, 128 registers
-// a thread; with a second column tile or 256 dims 168.
+// Warps of a CTA, its ring's stages and CTAs of an SM, by what the registers (64 dims: 80 a thread, 128 with a second
+// column tile; 128 dims: 128, 168 with it; 256 dims: 255) and 227 KB of shared memory hold.
 __host__ __device__ constexpr int ka_warps(int d, int nt) { return d == 128 && nt == 2 ? 12 : 8; }
 __host__ __device__ constexpr int ka_stages(int d, int nt) { return d == 64 ? (nt == 1 ? 4 : 6) : d == 128 && nt == 2 ? 4 : 3; }
 __host__ __device__ constexpr int ka_ctas(int d, int nt) { return d == 256 || (d == 128 && nt == 2) ? 1 : d == 64 && nt == 1 ? 3 : 2; }
 constexpr int kKaMaxCluster = 8;
-constexpr float kNoMax = -1e30f;
+constexpr float kNoMax = -3e38f;   // below every finite score's exponent
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -99,10 +106,10 @@ __device__ __forceinline__ uint32_t nonfinite_bytes(uint32_t w) {
 }
 
 // The line of tiles (below 2^31) of all segments, cut into parts, one for each CTA.
-// Few segments with few tiles (a.aligned): parts do not cross segments.  A segment of n
+// With at most half as many segments as CTAs (a.aligned) parts do not cross segments.  A segment of n
 // tiles has ceil(n / size) parts of nearly equal length; size = ceil(total / (CTAs - segments))
-// makes them at most as many as the CTAs.  A CTA that starts a second segment starts its pipeline
-// and merges again, about 4 us, which is worth more than the even shares when there are few tiles.
+// makes them at most as many as the CTAs.  A CTA that goes on to a second segment starts its pipeline and
+// merges again, about 4 us.
 // Otherwise all parts are of nearly equal length, the first `longer` of size + 1 tiles, the others of size.
 // Every part has a tile.
 struct Line {
@@ -142,7 +149,7 @@ struct Kv8Attn {
   struct Smem {
     union {
       uint8_t ring[kWarps][kStages][kTileBytes];  // 1024-byte aligned stages (the swizzle's period)
-      float o[kWarps][kRows][kOStride];           // the warps' sums, when the ring is empty; o[0], m[0], l[0] then the CTA's
+      float o[kWarps][kRows][kOStride];           // the warps' sums, when the ring is empty
     };
     float sent[kRows][D];                         // of the cluster's CTAs: [CTA][rows of this one]
     float2 sent_ml[kRows];
@@ -568,7 +575,8 @@ struct Kv8Attn {
       const int tok = __shfl_sync(0xffffffffu, now.tok, i & 31), exps = __shfl_sync(0xffffffffu, now.exps, i & 31);
       const uint32_t tile = ring + stage * kTileBytes;
       if (!__all_sync(0xffffffffu, bulk_wait(bars + 8 * stage, phase))) {
-        // never seen: the row would be wrong, so say so; the copies still in flight end before the CTA does
+        // The bounded wait ran out: the rows are incomplete, so say so and take no more tiles; the copies still
+        // in flight are waited for (again with a limit) before their memory is used otherwise.
         if (lane == 0 && a.status) atomicOr(a.status, MSKV_STATUS_TIMEOUT);
         for (int k = 0; k < kStages; ++k) bulk_wait(bars + 8 * k, phase);
         break;
@@ -1100,7 +1108,7 @@ static int check_attn(const mskv_kv8_attn_desc* d) {
   const int64_t most = d->blocks ? (int64_t)d->num_blocks * (d->pages.page_size / 16) : ((int64_t)d->max_tokens + 15) / 16;
   if (row_tiles * d->pages.batch * d->pages.kv_heads * most > INT_MAX / 2)
     return fail(MSKV_ERR_RANGE, "%s: too many tokens for one call", what);
-  if (!(fabsf(d->scale) <= 3e38f)) return fail(MSKV_ERR_ARG, "%s: scale must be finite", what);
+  if (!(fabsf(d->scale) <= 2e38f)) return fail(MSKV_ERR_ARG, "%s: scale must be finite", what);   // times log2(e) too
   return MSKV_OK;
 }
 

@@ -450,28 +450,35 @@ def test_large_offsets(built_lib):
     ops.check_status(torch.device("cuda"))
 
 
-def test_streams_and_graphs(built_lib):
-    """Calls on a side stream; two graphs of the same call on different inputs, replayed at the same time; a
-    graph replayed while the cache grows."""
+@pytest.mark.parametrize("tokens", [2000, 9000])        # a cluster for each segment; the line and its merge
+def test_streams_and_graphs(built_lib, tokens):
+    """Calls on a side stream; two streams at once; two graphs of the same call on different inputs, replayed at the
+    same time; a graph replayed while the cache grows."""
     from mserve_b200 import ops
     lens = [700, 1300]
-    pages, table, g = _filled(2, 2, 128, 16, E4M3, [2000, 2000], seed=21)
+    pages, table, g = _filled(2, 2, 128, 16, E4M3, [tokens, tokens], seed=21)
     table = table.cuda()
     qs = [torch.randn(2, 14, 1, 128, generator=g).to(torch.bfloat16).cuda() for _ in range(2)]
     n = _i32(lens)
-    want = [ops.kv8_attention(q, pages, table, lens=n, max_tokens=2000).clone() for q in qs]
+    want = [ops.kv8_attention(q, pages, table, lens=n, max_tokens=tokens).clone() for q in qs]
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
-    got = ops.kv8_attention(qs[0], pages, table, lens=n, max_tokens=2000, stream=side)
+    got = ops.kv8_attention(qs[0], pages, table, lens=n, max_tokens=tokens, stream=side)
     side.synchronize()
     assert torch.equal(got, want[0])
+    streams = [torch.cuda.Stream() for _ in qs]
+    torch.cuda.synchronize()
+    both = [[ops.kv8_attention(q, pages, table, lens=n, max_tokens=tokens, stream=st) for q, st in zip(qs, streams)]
+            for _ in range(10)]
+    torch.cuda.synchronize()
+    for pair in both:
+        assert torch.equal(pair[0], want[0]) and torch.equal(pair[1], want[1])
     graphs, outs = [], []
     for q in qs:
         gr = torch.cuda.CUDAGraph()
         with torch.cuda.graph(gr):
-            outs.append(ops.kv8_attention(q, pages, table, lens=n, max_tokens=2000))
+            outs.append(ops.kv8_attention(q, pages, table, lens=n, max_tokens=tokens))
         graphs.append(gr)
-    streams = [torch.cuda.Stream() for _ in qs]
     torch.cuda.synchronize()
     for _ in range(20):
         for gr, st in zip(graphs, streams):
@@ -480,12 +487,78 @@ def test_streams_and_graphs(built_lib):
     torch.cuda.synchronize()
     for o, w in zip(outs, want):
         assert torch.equal(o, w)
-    n.copy_(_i32([1999, 5]))
+    n.copy_(_i32([tokens - 1, 5]))
     graphs[0].replay()
-    assert torch.equal(outs[0], ops.kv8_attention(qs[0], pages, table, lens=n, max_tokens=2000))
+    assert torch.equal(outs[0], ops.kv8_attention(qs[0], pages, table, lens=n, max_tokens=tokens))
     torch.cuda.synchronize()
     ops.check_status(torch.device("cuda"))
     del graphs
+
+
+def test_captured_across_streams(built_lib):
+    """A graph whose streams fork and join between the calls: append on one, scores and attention on another."""
+    from mserve_b200 import ops
+    B, H, D, page = 2, 2, 128, 16
+    pages, table, g = _filled(B, H, D, page, E4M3, [500, 90], seed=51)
+    tab, tok0, n = table.cuda(), _i32([500, 90]), _i32([501, 91])
+    x = torch.randn(2, B, H, 1, D, generator=g).to(torch.bfloat16).cuda()
+    q = torch.randn(B, 14, 1, D, generator=g).to(torch.bfloat16).cuda()
+    scores = torch.zeros(B, H, tab.shape[1], device="cuda")
+    out = torch.zeros_like(q)
+    side = torch.cuda.Stream()
+
+    def work():
+        main = torch.cuda.current_stream()
+        ops.kv8_append(pages, tab, x[0], x[1], tok0=tok0)
+        side.wait_stream(main)
+        ops.kv8_block_score(q, pages, tab, lens=n, max_blocks=tab.shape[1], out=scores, stream=side)
+        ops.kv8_attention(q, pages, tab, lens=n, out=out, stream=side)
+        main.wait_stream(side)
+        return out + 1
+
+    work()
+    torch.cuda.synchronize()
+    want, s = out.clone(), scores.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plus = work()
+    for _ in range(5):
+        out.zero_()
+        scores.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(plus, want + 1) and torch.equal(scores, s)
+    ops.check_status(torch.device("cuda"))
+    del graph
+
+
+@pytest.mark.parametrize("D,Q", [(64, 1), (128, 1), (128, 4)])
+def test_bounds_far_above_the_lengths(built_lib, D, Q):
+    """A page table for a quarter of a million tokens with a few hundred in it: the work is split by the lengths."""
+    from mserve_b200 import ops
+    lens = [600, 0, 33, 599, 1, 350, 16, 17]
+    pages, table, g = _filled(8, 2, D, 16, E4M3, lens, seed=61)
+    wide = torch.full((8, 16000), -1, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    q = torch.randn(8, 14, Q, D, generator=g).to(torch.bfloat16)
+    want, bound = k8.attention(q.double(), _host(pages), table, lens)
+    _close(ops.kv8_attention(q.cuda(), pages, wide.cuda(), lens=_i32(lens)), want, bound)
+    ops.check_status(torch.device("cuda"))
+
+
+def test_attention_of_extreme_scores(built_lib):
+    """Scores of either sign far beyond what exp holds: a row whose scores are all very small is still a mean."""
+    from mserve_b200 import ops
+    pages, table, g = _filled(1, 1, 64, 16, E4M3, [80], seed=71)
+    host = _host(pages)
+    for size in (1e15, 1e30):
+        q = torch.zeros(1, 2, 1, 64)
+        q[0, 0, 0, 3], q[0, 1, 0, 3] = size, -size
+        q = q.to(torch.bfloat16)
+        want, _ = k8.attention(q.double(), host, table, [80])
+        got = ops.kv8_attention(q.cuda(), pages, table.cuda(), lens=_i32([80])).cpu().double()
+        # one token's weight is 1 (its score leads by more than 2^20 times the rounding of any): half a step of the output
+        assert ((got - want).abs() <= want.abs() * 2.0 ** -8).all()
 
 
 def test_results_do_not_vary(built_lib):
