@@ -3,7 +3,8 @@
 PyTorch supplies device memory, the current stream and dtypes; every byte of KV data is
 moved or reduced by the sm_100a kernels behind ``include/mserve_kv.h``.  Each wrapper
 validates shapes and strides on the host (raising ``ValueError``/``RuntimeError`` before any
-launch), fills the C descriptor and launches on ``torch.cuda.current_stream()``.
+launch), fills the C descriptor and launches on ``torch.cuda.current_stream()``; the kv8 calls do
+so in a torch extension (torch_ext/kv8_ops.cpp).
 """
 from __future__ import annotations
 

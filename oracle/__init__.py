@@ -8,6 +8,7 @@ only as the checker or as the timed CPU baseline -- never as part of the product
 Contents
   kv_oracle.py    numpy restatement, one function per reference step, each citing the
                   reference file:line it follows (qwen-eljrte/...).
+  kv8_oracle.py   64-bit restatement of the 8-bit paged cache (no reference counterpart).
   oracle_kv.c     the same gather / scoring / top-k / attention in plain C + OpenMP, used as
                   the timed CPU baseline (built into liboracle_kv.so by build_oracle.py).
   build_oracle.py gcc recipe for liboracle_kv.so.
