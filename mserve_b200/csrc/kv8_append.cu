@@ -414,8 +414,9 @@ extern "C" int mskv_kv8_append(const mskv_kv8_append_desc* d, void* stream) {
   a.touched = (uint32_t)(((int64_t)d->num_tokens + a.pg.page_size - 2) / a.pg.page_size + 1);
   const int64_t all = (int64_t)a.touched * a.pg.batch * a.pg.heads;
   a.all_units = (uint32_t)all;
-  // Units of 2 * page_size/16 warps: up to 8 warps a CTA, but one unit each while every SM has room for them
-  // (a decode token of 8 sequences, 4 heads: 2.7 us against 3.3).
+  // Few units: one a CTA and all of a page's rows loaded together; more: up to 8 warps a CTA, in fewer registers.  128 dims,
+  // bf16, pages of 16: 32 units 3.4 us against 4.8, 576 units 4.1 against 5.8, 1088 units 7.2 against 6.4, 2176
+  // units 14.5 against 8.7.
   const bool few = all <= 4 * (int64_t)sms_of_device();
   a.units = few ? 1 : (uint32_t)std::max(1, 64 / a.pg.page_size);
   const int64_t ctas = (all + a.units - 1) / a.units;

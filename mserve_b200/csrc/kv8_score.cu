@@ -205,8 +205,9 @@ extern "C" int mskv_kv8_block_score(const mskv_kv8_score_desc* d, void* stream) 
   a.status = d->status;
   a.group = d->q_heads / d->pages.kv_heads;
   a.max_blocks = d->max_blocks;
-  // Tiles a warp takes per CTA: one while that fits one wave of the GPU, up to four beyond, so the
-  // weights' set-up is shared.
+  // Tiles a warp takes per CTA: one while that fits one wave of the GPU, up to four beyond, so that the weights' set-up is
+  // shared.  One, two, four, eight: 8 sequences of 1024 pages, 4 heads 4.9, 5.8, 7.7, 11.3 us; 16 of 2048, 8 heads
+  // 20.0, 16.6, 14.7, 15.5 us; 64 of 256, 4 heads 6.8, 7.2, 7.2, 7.3 us.
   const int64_t segs = (int64_t)a.pg.batch * a.pg.heads;
   const int64_t rows = ((int64_t)d->max_blocks + 16 * kBsWarps - 1) / (16 * kBsWarps);
   a.tiles = (int)std::min<int64_t>(4, std::max<int64_t>(1, segs * rows / (2 * sms_of_device())));
