@@ -108,10 +108,16 @@ __device__ __forceinline__ void row_values(bool old, const uint32_t (&w)[NT == k
 
 template <bool E5M2>
 __device__ __forceinline__ void store_codes(uint8_t* p, const float (&x)[8], float inv) {
-  uint2 c;
-  c.x = to_codes<E5M2>(x[0] * inv, x[1] * inv) | (to_codes<E5M2>(x[2] * inv, x[3] * inv) << 16);
-  c.y = to_codes<E5M2>(x[4] * inv, x[5] * inv) | (to_codes<E5M2>(x[6] * inv, x[7] * inv) << 16);
-  *reinterpret_cast<uint2*>(p) = c;
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    // a packed product of two
+    float a, b;
+    asm("{ .reg .b64 v, k; mov.b64 v, {%2, %3}; mov.b64 k, {%4, %4}; mul.rn.f32x2 v, v, k; mov.b64 {%0, %1}, v; }"
+        : "=f"(a), "=f"(b) : "f"(x[2 * i]), "f"(x[2 * i + 1]), "f"(inv));
+    w[i] = to_codes<E5M2>(a, b);
+  }
+  *reinterpret_cast<uint2*>(p) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
 }
 
 template <typename H2>
@@ -150,6 +156,113 @@ __device__ __forceinline__ int exponent_for(uint32_t a) {
   if (!a) return MSKV_KV8_EXP_MIN;
   const int e = (int)(a >> 23) - 127 - (E5M2 ? 15 : 8) + ((a & 0x7fffffu) > 0x600000u);
   return min(max(e, MSKV_KV8_EXP_MIN), MSKV_KV8_EXP_MAX);
+}
+
+// A page (one half, one warp's 16 rows of it) that only receives new 16-bit rows.  A lane takes 16 elements of a row and
+// step, eight from each half of the row, packed in pairs.
+template <int D, bool E5M2, int NT, bool VEC>
+__device__ __forceinline__ void new_page(const char* rows0, int64_t stride, uint8_t* codes, int8_t* ex, uint8_t* bounds, int rows,
+                                         int kv, int parts, int part, int bar, uint32_t* slots, uint32_t* slots2,
+                                         float* s_lo, float* s_hi, int lane) {
+  using H2 = std::conditional_t<NT == kNewBf16, __nv_bfloat162, __half2>;
+  constexpr uint32_t kInf = NT == kNewBf16 ? 0x7f80u : 0x7c00u;
+  constexpr int kLanes = D / 16, kRows = 32 / kLanes, kSteps = 16 / kRows;
+  const int r0 = part * 16 + lane / kLanes, c = (lane % kLanes) * 8;
+  const char* src = rows0 + r0 * stride + c * 2;
+  uint32_t x[kSteps][8];
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s)
+    if (r0 + s * kRows < rows) {
+      load8_packed<VEC>(src + s * kRows * stride, *reinterpret_cast<uint32_t(*)[4]>(&x[s][0]));
+      load8_packed<VEC>(src + s * kRows * stride + D, *reinterpret_cast<uint32_t(*)[4]>(&x[s][4]));
+    }
+  // the lane's columns: their bounds, and of those the largest magnitude (NaN and infinities stay visible)
+  H2 lo[8], hi[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    lo[i] = as_pair<H2>(kInf * 0x10001u);
+    hi[i] = as_pair<H2>(kInf * 0x10001u | 0x80008000u);
+  }
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s)
+    if (r0 + s * kRows < rows)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        lo[i] = __hmin2_nan(lo[i], as_pair<H2>(x[s][i]));
+        hi[i] = __hmax2_nan(hi[i], as_pair<H2>(x[s][i]));
+      }
+  uint32_t top = 0;
+  if (r0 < rows) {
+    H2 most = as_pair<H2>(0u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = __hmax2_nan(most, __hmax2_nan(__habs2(lo[i]), __habs2(hi[i])));
+    const uint32_t both = *reinterpret_cast<const uint32_t*>(&most) & 0x7fff7fffu;   // NaN: all ones
+    top = max(both >> 16, both & 0xffffu);
+  }
+  top = half_max(top, slots, bar, parts, part, lane);
+  if (top >= kInf) {                        // infinities or NaN: the maximum of the others
+    uint32_t both = 0;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+      if (r0 + s * kRows < rows)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t m = x[s][i] & 0x7fff7fffu;
+          both = __vmaxu2(both, m & __vcmpltu2(m, kInf * 0x10001u));
+        }
+    top = half_max(max(both >> 16, both & 0xffffu), slots2, bar, parts, part, lane);
+  }
+  const int e = exponent_for<E5M2>(NT == kNewBf16 ? top << 16 : __float_as_uint(__half2float(__ushort_as_half((uint16_t)top))));
+  const float inv = pow2i(-e);
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s)
+    if (r0 + s * kRows < rows) {
+      uint8_t* dst = codes + (r0 + s * kRows) * D + c;
+      float f[8];
+      unpack8<NT>(*reinterpret_cast<const uint32_t(*)[4]>(&x[s][0]), f);
+      store_codes<E5M2>(dst, f, inv);
+      unpack8<NT>(*reinterpret_cast<const uint32_t(*)[4]>(&x[s][4]), f);
+      store_codes<E5M2>(dst + D / 2, f, inv);
+    }
+  if (part == 0 && lane == 0) *ex = (int8_t)e;
+  if (kv || !bounds) return;
+#pragma unroll
+  for (int o = kLanes; o < 32; o <<= 1)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      lo[i] = __hmin2_nan(lo[i], __shfl_xor_sync(0xffffffffu, lo[i], o));
+      hi[i] = __hmax2_nan(hi[i], __shfl_xor_sync(0xffffffffu, hi[i], o));
+    }
+  if (lane >= kLanes && parts == 1) return;
+  float l[16], m[16];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    l[2 * i] = __low2float(lo[i]); l[2 * i + 1] = __high2float(lo[i]);
+    m[2 * i] = __low2float(hi[i]); m[2 * i + 1] = __high2float(hi[i]);
+  }
+  if (parts > 1) {
+    if (lane < kLanes)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int d = part * D + (i >> 3) * (D / 2) + c + (i & 7);
+        s_lo[d] = l[i];
+        s_hi[d] = m[i];
+      }
+    half_barrier(bar, parts);
+    if (part || lane >= kLanes) return;
+    for (int q = 1; q < parts; ++q)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int d = q * D + (i >> 3) * (D / 2) + c + (i & 7);
+        l[i] = min_nan(l[i], s_lo[d]);
+        m[i] = max_nan(m[i], s_hi[d]);
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    store_codes<E5M2>(bounds + i * (D / 2) + c, *reinterpret_cast<const float(*)[8]>(&l[8 * i]), inv);
+    store_codes<E5M2>(bounds + D + i * (D / 2) + c, *reinterpret_cast<const float(*)[8]>(&m[8 * i]), inv);
+  }
 }
 
 // kFew: few units (see the launch).  Every page's rows then go through fp32 and are loaded together (eight steps;
@@ -212,69 +325,16 @@ __global__ void __launch_bounds__(512, !kFew && D <= 128 && NT != kNewF32 ? 2 : 
     lo[i] = INFINITY;
     hi[i] = -INFINITY;
   }
-  if (NT != kNewF32 && !kFew && first_new == 0) {
-    using H2 = std::conditional_t<NT == kNewBf16, __nv_bfloat162, __half2>;
-    constexpr uint32_t kInf = NT == kNewBf16 ? 0x7f80u : 0x7c00u;
-    uint32_t x[kSteps][4];
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[s][i] = 0u;
-      if (r0 + s * kRows < rows) load8_packed<VEC>(src + s * step, x[s]);
+  if constexpr (NT != kNewF32 && !kFew) {
+    if (first_new == 0) {
+      const char* rows0 = a.x[kv] + (int64_t)b * a.sb[kv] + (int64_t)h * a.sh[kv] + (t0 - tok0) * a.st[kv];
+      new_page<D, E5M2, NT, VEC>(rows0, a.st[kv], codes, ex, a.pg.bounds ? a.pg.bounds + (page * a.pg.heads + h) * 2 * D : nullptr,
+                                 rows, kv, parts, part, bar, s_max[0] + warp - part, s_max[1] + warp - part, s_lo[group * parts],
+                                 s_hi[group * parts], lane);
+      return;
     }
-    H2 most = as_pair<H2>(0u);
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) most = __hmax2_nan(most, __habs2(as_pair<H2>(x[s][i])));
-    uint32_t both = *reinterpret_cast<const uint32_t*>(&most) & 0x7fff7fffu;   // NaN: all ones
-    uint32_t top = half_max(max(both >> 16, both & 0xffffu), s_max[0] + warp - part, bar, parts, part, lane);
-    if (top >= kInf) {                      // infinities or NaN: the maximum of the others
-      both = 0;
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t m = x[s][i] & 0x7fff7fffu;
-          both = __vmaxu2(both, m & __vcmpltu2(m, kInf * 0x10001u));
-        }
-      top = half_max(max(both >> 16, both & 0xffffu), s_max[1] + warp - part, bar, parts, part, lane);
-    }
-    const int e = exponent_for<E5M2>(NT == kNewBf16 ? top << 16 : __float_as_uint(__half2float(__ushort_as_half((uint16_t)top))));
-    const float inv = pow2i(-e);
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      const int r = r0 + s * kRows;
-      if (r < rows) {
-        float f[8];
-        unpack8<NT>(x[s], f);
-        store_codes<E5M2>(codes + (int64_t)r * D + d0, f, inv);
-      }
-    }
-    if (part == 0 && lane == 0) *ex = (int8_t)e;
-    if (!a.pg.bounds) return;               // the same for every thread of the launch
-    if (kv == 0) {
-      H2 l2[4], h2[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        l2[i] = as_pair<H2>(kInf * 0x10001u);
-        h2[i] = as_pair<H2>(kInf * 0x10001u | 0x80008000u);
-      }
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s)
-        if (r0 + s * kRows < rows)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            l2[i] = __hmin2_nan(l2[i], as_pair<H2>(x[s][i]));
-            h2[i] = __hmax2_nan(h2[i], as_pair<H2>(x[s][i]));
-          }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        lo[2 * i] = __low2float(l2[i]) * inv; lo[2 * i + 1] = __high2float(l2[i]) * inv;
-        hi[2 * i] = __low2float(h2[i]) * inv; hi[2 * i + 1] = __high2float(h2[i]) * inv;
-      }
-    }
-  } else {
+  }
+  {
     const float f_old = pow2i(e_old);
     // a batch of steps: their loads, then their values
     constexpr int kMost = kFew && NT != kNewF32 ? 8 : 4, kBatch = kSteps < kMost ? kSteps : kMost;
