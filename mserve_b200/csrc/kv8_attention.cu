@@ -66,8 +66,8 @@ struct Kv8AttnDev {
   float* part_o;                   // [2 * CTAs][rows][D]
   uint32_t* status;
   float scale_log2;
-  int32_t group, q_len, rows, row_tiles, segments, max_tokens, width, cluster;   // cluster: CTAs that share a segment, 0: the line
-  int32_t vec_q, pow2_page, aligned;
+  int32_t group, q_len, rows, row_tiles, segments, max_tokens, width, cluster;   // cluster: CTAs that share a segment (1, 2, 4, 8), 0: the line
+  int32_t cluster_log2, vec_q, pow2_page, aligned;
 };
 
 // Warps of a CTA, its ring's stages and CTAs of an SM, by what the registers (64 dims: 80 a thread, 128 with a second
@@ -167,6 +167,9 @@ struct Kv8Attn {
   float m[NT][2], l[NT][2];
   float o[NT][kOT][4];
 
+  // Query position of row r of a KV head.
+  static __device__ __forceinline__ int position(const Kv8AttnDev& a, int r) { return a.q_len == 1 ? 0 : r / a.group; }
+
   // Query rows of the segment to shared memory, in two steps, so that the codes' first loads come between: a
   // warp takes rows warp and warp + kWarps (two column tiles), a lane D/32 neighbouring elements of each.
   // Row 8*(row tile*NT + nt) + n is position * group + head.
@@ -182,7 +185,7 @@ struct Kv8Attn {
 #pragma unroll
       for (int i = 0; i < kQPer / 2; ++i) q.w[k][i] = 0u;
       if (n < kRows && r < a.rows) {
-        const int pos = r / a.group, head = h * a.group + r - pos * a.group;
+        const int pos = position(a, r), head = h * a.group + r - pos * a.group;
         const char* src = a.q + (int64_t)b * a.q_sb + (int64_t)head * a.q_sh + (int64_t)pos * a.q_sq + lane * (kQPer * 2);
         if (!a.vec_q) {
           const uint16_t* u = reinterpret_cast<const uint16_t*>(src);
@@ -225,7 +228,7 @@ struct Kv8Attn {
         *reinterpret_cast<uint32_t*>(&sm.q[n][lane * kQPer + i]) = pack_half2(x[i] * inv, x[i + 1] * inv);
       if (lane == 0) {
         sm.f[n] = a.scale_log2 * pow2i(e);
-        sm.lim[n] = len - a.q_len + 1 + (r < a.rows ? r / a.group : a.q_len - 1);
+        sm.lim[n] = len - a.q_len + 1 + (r < a.rows ? position(a, r) : a.q_len - 1);
       }
     }
   }
@@ -275,8 +278,11 @@ struct Kv8Attn {
   // Tile `i` of (b, h) as one lane sees it.
   static __device__ __forceinline__ Tile find(const Kv8AttnDev& a, int b, int h, int len, int i) {
     const int parts = a.pg.page_size >> 4;
-    int pi = i / parts;
-    const int part = i - pi * parts;
+    int pi = i, part = 0;
+    if (parts > 1) {
+      pi = i / parts;
+      part = i - pi * parts;
+    }
     Tile t;
     t.page = -1;
     t.tok = 0;
@@ -679,18 +685,18 @@ struct Kv8Attn {
   // The same for a cluster of `ctas` CTAs that share a segment: every CTA stores its sums of row r into the shared
   // memory of CTA r % ctas, which finishes the row after one barrier of the cluster (nothing reads another
   // CTA's memory after that, so each may end).
-  static __device__ __forceinline__ void finish_cluster(const Kv8AttnDev& a, Smem& sm, const Place& at, int rank, int ctas) {
+  static __device__ __forceinline__ void finish_cluster(const Kv8AttnDev& a, Smem& sm, const Place& at, int rank, int ctas, int log2) {
     cg::cluster_group cluster = cg::this_cluster();
     cluster.barrier_wait();                       // all CTAs of the cluster run (they arrived when they began)
 #pragma unroll 1
     for (int i = threadIdx.x; i < kRows * D / 4; i += kThreads) {
-      const int r = i / (D / 4), d = (i % (D / 4)) * 4, owner = r % ctas, slot = rank * ((kRows + ctas - 1) / ctas) + r / ctas;
+      const int r = i / (D / 4), d = (i % (D / 4)) * 4, owner = r & (ctas - 1), slot = rank * (kRows >> log2) + (r >> log2);
       const Part y = cta_part(sm, r, d);
       *cluster.map_shared_rank(reinterpret_cast<float4*>(&sm.sent[slot][d]), owner) = y.x;
       if (d == 0) *cluster.map_shared_rank(&sm.sent_ml[slot], owner) = make_float2(y.top, y.sum);
     }
     cluster.sync();
-    const int each = (kRows + ctas - 1) / ctas;   // rows of a CTA; a row is a stretch of D/4 threads
+    const int each = kRows >> log2;               // rows of a CTA; a row is a stretch of D/4 threads
     const int stretch = threadIdx.x / (D / 4), d = (threadIdx.x % (D / 4)) * 4;
 #pragma unroll 1
     for (int k = stretch; k < each; k += kThreads / (D / 4)) {
@@ -714,7 +720,7 @@ struct Kv8Attn {
 
   // out[row][d .. d+3] = x / sum, 0 for a row that saw nothing.
   static __device__ __forceinline__ void write_out(const Kv8AttnDev& a, int b, int h, int r, int d, float4 x, float sum) {
-    const int pos = r / a.group, head = h * a.group + r % a.group;
+    const int pos = position(a, r), head = h * a.group + r - pos * a.group;
     char* dst = a.out + (int64_t)b * a.o_sb + (int64_t)head * a.o_sh + (int64_t)pos * a.o_sq + d * 2;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     const float y[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
@@ -828,15 +834,15 @@ kv8_attn_kernel(const Kv8AttnDev a, const __grid_constant__ CUtensorMap k_map, c
   if (a.cluster) {
     // the CTAs of a cluster share a segment, and need not know the others
     if (threadIdx.x == 0) {
-      const uint32_t rank = blockIdx.x % a.cluster, seg = blockIdx.x / a.cluster;
-      const int bh = (int)(seg / a.row_tiles);
-      at.rt = (int)(seg % a.row_tiles);
+      const uint32_t rank = blockIdx.x & (a.cluster - 1), seg = blockIdx.x >> a.cluster_log2;
+      const int bh = a.row_tiles == 1 ? (int)seg : (int)(seg / a.row_tiles);
+      at.rt = (int)(seg - bh * a.row_tiles);
       at.b = bh / a.pg.heads;
       at.h = bh - at.b * a.pg.heads;
       at.len = kv8_len(a, at.b);
       at.n = kv8_tiles(a, at.b, at.h);
       at.start = 0;
-      const uint32_t share = at.n / a.cluster, longer = at.n - share * a.cluster;
+      const uint32_t share = at.n >> a.cluster_log2, longer = at.n & (a.cluster - 1);
       at.begin = at.at = rank * share + min(rank, longer);
       at.end = at.at + share + (rank < longer ? 1 : 0);
     }
@@ -853,7 +859,7 @@ kv8_attn_kernel(const Kv8AttnDev a, const __grid_constant__ CUtensorMap k_map, c
   for (;;) {
     k.piece(a, &k_map, &v_map, sm, at, turn, warp, lane);
     if (a.cluster > 1) {
-      K::finish_cluster(a, sm, at, blockIdx.x % a.cluster, a.cluster);
+      K::finish_cluster(a, sm, at, (int)(blockIdx.x & (a.cluster - 1)), a.cluster, a.cluster_log2);
       return;
     }
     const uint32_t first = at.at - at.start, last = min(at.n, at.end - at.start);
@@ -1156,6 +1162,7 @@ extern "C" int mskv_kv8_attention(const mskv_kv8_attn_desc* d, void* stream) {
   a.max_tokens = d->max_tokens;
   a.width = d->num_blocks;
   a.cluster = p.cluster;
+  for (a.cluster_log2 = 0; (2 << a.cluster_log2) <= p.cluster; ++a.cluster_log2) {}
   a.aligned = p.aligned;
   a.vec_q = (q_bits & 15) == 0;
   a.pow2_page = (a.pg.page_size & (a.pg.page_size - 1)) == 0;
