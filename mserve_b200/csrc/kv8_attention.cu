@@ -66,8 +66,10 @@ struct Kv8AttnDev {
   float* part_o;                   // [2 * CTAs][rows][D]
   uint32_t* status;
   float scale_log2;
-  int32_t group, q_len, rows, row_tiles, segments, max_tokens, width, cluster;   // cluster: CTAs that share a segment (1, 2, 4, 8), 0: the line
-  int32_t cluster_log2, vec_q, pow2_page, aligned;
+  int32_t group, q_len, rows, row_tiles, segments, max_tokens, width;
+  int32_t cluster, cluster_log2;   // CTAs that share a segment (1, 2, 4, 8); 0: the line
+  int32_t parts_log2;              // tiles of a page; -1 where they are no power of two
+  int32_t vec_q, pow2_page, aligned;
 };
 
 // Warps of a CTA, its ring's stages and CTAs of an SM, by what the registers (64 dims: 80 a thread, 128 with a second
@@ -278,11 +280,8 @@ struct Kv8Attn {
   // Tile `i` of (b, h) as one lane sees it.
   static __device__ __forceinline__ Tile find(const Kv8AttnDev& a, int b, int h, int len, int i) {
     const int parts = a.pg.page_size >> 4;
-    int pi = i, part = 0;
-    if (parts > 1) {
-      pi = i / parts;
-      part = i - pi * parts;
-    }
+    int pi = a.parts_log2 >= 0 ? i >> a.parts_log2 : i / parts;
+    const int part = i - pi * parts;
     Tile t;
     t.page = -1;
     t.tok = 0;
@@ -1162,6 +1161,8 @@ extern "C" int mskv_kv8_attention(const mskv_kv8_attn_desc* d, void* stream) {
   a.max_tokens = d->max_tokens;
   a.width = d->num_blocks;
   a.cluster = p.cluster;
+  const int parts = a.pg.page_size / 16;
+  a.parts_log2 = parts & (parts - 1) ? -1 : parts >= 8 ? 3 : parts >> 1;
   for (a.cluster_log2 = 0; (2 << a.cluster_log2) <= p.cluster; ++a.cluster_log2) {}
   a.aligned = p.aligned;
   a.vec_q = (q_bits & 15) == 0;
