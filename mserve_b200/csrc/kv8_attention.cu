@@ -34,8 +34,8 @@
 // lengths in every CTA); a segment of several parts goes through the workspace and a second kernel.
 //
 // Measured (device time, three sets of inputs in turn): 40/8 heads, 128 dims, 16 sequences of 32768 tokens
-// (1.07 GB) 173 us = 0.95 of the copy rate; 28/4 heads, 8 of 16384 (134 MB) 28.3 us = 0.73, of which 4.5 us pass
-// before the first codes are there and 3 after the last; 136 listed pages of each (18 MB) 9.3 us.
+// (1.07 GB) 172 us = 0.95 of the copy rate; 28/4 heads, 8 of 16384 (134 MB) 27.6 us = 0.75, of which 3 us pass
+// before the first codes are there and 2 after the last; 136 listed pages of each (18 MB) 8.8 us.
 // Loads straight into registers instead of the ring (one tile ahead, as many as the registers hold): 181,
 // 32.5 and 11.7 us, and 10% more than that at the clocks of a GPU at its power limit; the same chunks through
 // cp.async into a ring: 257 us for the first.
@@ -996,21 +996,26 @@ static Kv8Plan make_plan(const mskv_kv8_attn_desc& d) {
   const int64_t most = d.blocks ? (int64_t)d.num_blocks * (d.pages.page_size / 16) : ((int64_t)d.max_tokens + 15) / 16;
   const int warps = ka_warps(d.pages.head_dim, p.nt);
   const int64_t slots = (int64_t)sms_of_device() * ka_ctas(d.pages.head_dim, p.nt);   // CTAs that run at once
-  // A cluster of 1 to 8 CTAs for each segment, merged in its shared memory: no line to find one's place on, no
-  // second kernel, but the segments wait for the longest.  Chosen
-  //  * for short segments (up to four tiles a warp), with two tiles a warp or less;
-  //  * where the clusters fill four fifths of the GPU or more and all of it at most (at two thirds, 32/8 heads of 64
-  //    dims, 4 positions, 6 ragged sequences: 26.5 us against 19.4): for lists, which are of one
-  //    length as a rule, and for up to 32 tiles a warp: 28/4 heads, 8 sequences of 16384 tokens 28.1 us against
-  //    32.4 on the line, 16 of 4096 17.7 against 20.8, 64 of up to 4096 41.2 against 46.1; ragged down to an
-  //    eighth, 8 of up to 16384: 23.5 against 22.7.  Longer ones not: 40/8 heads, 16 of 32768, ragged: 144 us in
-  //    clusters of two, 107 on the line (equal lengths: 175 and 173).
-  int cluster = 1, fill = 1;
+  // A cluster of 1 to 8 CTAs for each segment, merged in its shared memory, spares the line's look-up and the second
+  // kernel (4 us, and 4 more where parts would cross segments), but the segments wait for the longest: its tiles a
+  // warp, at the time that one takes on an SM of its own.  It is chosen while that is less than what the codes take
+  // at 6.3 TB/s, as far as the clusters fill the GPU, and those 4 us; of whole caches, whose lengths may differ, 0.85
+  // of the codes' time and 25 us at most are counted (lists are of one length as a rule).  A cluster has two tiles
+  // a warp or fewer and all clusters run at once.  Measured, cluster / line: 28/4 heads, 8 sequences of 16384 tokens
+  // 28.0 / 31.6 us (ragged down to an eighth 23.1 / 22.0), 16 of 4096 17.0 / 20.8, 64 of up to 4096 41.2 / 46.1, 4 of
+  // 32768 41.0 / 31.7, 5 of up to 9000 14.2 / 11.6; 40/8 heads, 30 of up to 2900 30.3 / 36.4, 16 of 32768 175 / 173, ragged
+  // 144 / 107; 8/1 heads of 256 dims, 2 positions, 46 of 846 13.5 / 19.5; 32/8 heads of 64 dims, 4 positions, 6 of up to
+  // 9001 25.7 / 20.2; lists of 516 pages, 40/8 heads, 10 sequences 43.7 / 40.2, of 208, 32/8
+  // heads of 64 dims, 8 sequences 14.1 / 15.4.
+  const int d_of = d.pages.head_dim;
+  const double tile_us = d_of == 64 ? 0.73 : d_of == 256 ? 1.14 : p.nt == 1 ? 0.84 : 1.25;
+  const double codes_us = (double)p.segments * most * 32 * d_of / 6.3e6;
+  int cluster = 1;
   while (cluster < kKaMaxCluster && most > 2 * warps * cluster && p.segments * cluster * 2 <= slots) cluster *= 2;
-  while (fill < kKaMaxCluster && p.segments * fill * 2 <= slots) fill *= 2;
-  const bool fills = p.segments * fill <= slots && p.segments * fill * 5 >= slots * 4;
-  if (most > 4 * warps * cluster && fills && (d.blocks || most <= 32 * warps * fill)) cluster = fill;
-  if (most <= 4 * warps * cluster || (fills && cluster == fill && (d.blocks || most <= 32 * warps * fill))) {
+  const double alone_us = tile_us * ((most + warps * cluster - 1) / (warps * cluster));
+  const double fill = (double)p.segments * cluster / slots;
+  const double line_us = fill * (d.blocks ? codes_us : std::min(0.85 * codes_us, 25.0)) + (p.segments * 2 > slots ? 8 : 4);
+  if (most <= 4 * warps * cluster || (fill <= 1 && alone_us <= line_us)) {
     p.cluster = cluster;
     p.ctas = p.segments * cluster;
     return p;
