@@ -43,6 +43,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "kv8.cuh"
 #include "tensor_map.cuh"
@@ -987,6 +988,59 @@ struct Kv8Plan {
   uint64_t info_bytes, ml_bytes, o_bytes;
 };
 
+template <int D, int NT>
+constexpr int ka_smem() {
+  return (int)sizeof(typename Kv8Attn<D, NT, false, true>::Smem) + 1024;   // + the ring's alignment
+}
+
+// A launch of `ctas` CTAs in clusters; `attrs` must outlive the configuration.
+template <int D, int NT>
+static cudaLaunchConfig_t ka_config(cudaLaunchAttribute (&attrs)[2], int64_t ctas, int cluster, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(32 * ka_warps(D, NT));
+  cfg.dynamicSmemBytes = ka_smem<D, NT>();
+  cfg.stream = st;
+  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  attrs[1].id = cudaLaunchAttributeClusterDimension;
+  attrs[1].val.clusterDim.x = (unsigned)std::max(cluster, 1);
+  attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
+  cfg.attrs = attrs;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cfg;
+}
+
+// Clusters of 2^log2 CTAs that run at once: fewer than the CTAs that do, as a cluster lies within one group of
+// multiprocessors (33 of 8 instead of 37 at 128 dims).  Asked for once per device and shape.
+template <int D, int NT>
+static int64_t clusters_at_once(int log2, int64_t slots) {
+  static std::atomic<int> known[64][4];
+  int dev = 0;
+  if (log2 == 0 || cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return slots >> log2;
+  int n = known[dev][log2].load(std::memory_order_relaxed);
+  if (n == 0) {
+    const auto kernel = kv8_attn_kernel<D, NT, false, true>;
+    cudaLaunchAttribute attrs[2];
+    cudaLaunchConfig_t cfg = ka_config<D, NT>(attrs, slots >> log2 << log2, 1 << log2, nullptr);
+    cfg.attrs = attrs + 1;
+    cfg.numAttrs = 1;
+    if (ensure_smem_limit(reinterpret_cast<const void*>(kernel), ka_smem<D, NT>(), "mskv_kv8_attention") ||
+        cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
+      cudaGetLastError();
+      return slots >> log2;
+    }
+    known[dev][log2].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+static int64_t clusters_at_once(int d, int nt, int log2, int64_t slots) {
+  if (d == 256) return clusters_at_once<256, 1>(log2, slots);
+  if (d == 128) return nt == 1 ? clusters_at_once<128, 1>(log2, slots) : clusters_at_once<128, 2>(log2, slots);
+  return nt == 1 ? clusters_at_once<64, 1>(log2, slots) : clusters_at_once<64, 2>(log2, slots);
+}
+
 static Kv8Plan make_plan(const mskv_kv8_attn_desc& d) {
   Kv8Plan p{};
   const int rows = d.q_heads / d.pages.kv_heads * d.q_len;
@@ -1001,7 +1055,7 @@ static Kv8Plan make_plan(const mskv_kv8_attn_desc& d) {
   // warp, at the time that one takes on an SM of its own.  It is chosen while that is less than what the codes take
   // at 6.3 TB/s, as far as the clusters fill the GPU, and those 4 us; of whole caches, whose lengths may differ, 0.85
   // of the codes' time and 25 us at most are counted (lists are of one length as a rule).  A cluster has two tiles
-  // a warp or fewer and all clusters run at once.  Measured, cluster / line: 28/4 heads, 8 sequences of 16384 tokens
+  // a warp or fewer where all clusters run at once.  Measured, cluster / line: 28/4 heads, 8 sequences of 16384 tokens
   // 28.0 / 31.6 us (ragged down to an eighth 23.1 / 22.0), 16 of 4096 17.0 / 20.8, 64 of up to 4096 41.2 / 46.1, 4 of
   // 32768 41.0 / 31.7, 5 of up to 9000 14.2 / 11.6; 40/8 heads, 30 of up to 2900 30.3 / 36.4, 16 of 32768 175 / 173, ragged
   // 144 / 107; 8/1 heads of 256 dims, 2 positions, 46 of 846 13.5 / 19.5; 32/8 heads of 64 dims, 4 positions, 6 of up to
@@ -1011,7 +1065,10 @@ static Kv8Plan make_plan(const mskv_kv8_attn_desc& d) {
   const double tile_us = d_of == 64 ? 0.73 : d_of == 256 ? 1.14 : p.nt == 1 ? 0.84 : 1.25;
   const double codes_us = (double)p.segments * most * 32 * d_of / 6.3e6;
   int cluster = 1;
-  while (cluster < kKaMaxCluster && most > 2 * warps * cluster && p.segments * cluster * 2 <= slots) cluster *= 2;
+  for (int log2 = 1; (1 << log2) <= kKaMaxCluster && most > 2 * warps * cluster; ++log2) {
+    if (p.segments > clusters_at_once(d_of, p.nt, log2, slots)) break;
+    cluster = 1 << log2;
+  }
   const double alone_us = tile_us * ((most + warps * cluster - 1) / (warps * cluster));
   const double fill = (double)p.segments * cluster / slots;
   const double line_us = fill * (d.blocks ? codes_us : std::min(0.85 * codes_us, 25.0)) + (p.segments * 2 > slots ? 8 : 4);
@@ -1052,25 +1109,14 @@ static bool encode_pages_map(CUtensorMap* m, uint8_t* base, const Kv8Dev& pg, in
 
 template <int D, int NT, bool E5M2, bool BF16>
 static int launch_attn(const Kv8AttnDev& a, const Kv8Plan& p, cudaStream_t st) {
-  constexpr int smem = (int)sizeof(typename Kv8Attn<D, NT, E5M2, BF16>::Smem) + 1024;   // + the ring's alignment
+  static_assert(sizeof(typename Kv8Attn<D, NT, E5M2, BF16>::Smem) == sizeof(typename Kv8Attn<D, NT, false, true>::Smem));
   const auto kernel = kv8_attn_kernel<D, NT, E5M2, BF16>;
-  if (const int rc = ensure_smem_limit(reinterpret_cast<const void*>(kernel), smem, "mskv_kv8_attention")) return rc;
+  if (const int rc = ensure_smem_limit(reinterpret_cast<const void*>(kernel), ka_smem<D, NT>(), "mskv_kv8_attention")) return rc;
   CUtensorMap maps[2];
   if (!encode_pages_map(&maps[0], a.pg.k, a.pg, D) || !encode_pages_map(&maps[1], a.pg.v, a.pg, D))
     return fail(MSKV_ERR_CUDA, "mskv_kv8_attention: the cache's layout cannot be encoded for TMA");
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)p.ctas);
-  cfg.blockDim = dim3(32 * ka_warps(D, NT));
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = (unsigned)std::max(p.cluster, 1);
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = p.cluster > 1 ? 2 : 1;
+  cudaLaunchAttribute attrs[2];
+  const cudaLaunchConfig_t cfg = ka_config<D, NT>(attrs, p.ctas, p.cluster, st);
   const cudaError_t launched = cudaLaunchKernelEx(&cfg, kernel, a, maps[0], maps[1]);
   if (launched != cudaSuccess) return cuda_status(launched, "mskv_kv8_attention launch");
   if (const int rc = after_launch("mskv_kv8_attention")) return rc;
