@@ -23,6 +23,21 @@
 
 namespace mskv {
 
+// Division by an invariant (Granlund and Montgomery): a multiplication, an average and a shift.
+struct Divisor {
+  uint32_t factor, shift;
+  explicit Divisor(uint32_t d = 1) : factor(1), shift(0) {
+    uint32_t l = 0;
+    while (l < 32 && ((uint64_t)1 << l) < d) ++l;
+    factor = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << l) - d)) / d + 1);
+    shift = l;
+  }
+  __device__ __forceinline__ uint32_t quotient(uint32_t n) const {
+    const uint32_t t = __umulhi(factor, n);
+    return shift ? (t + ((n - t) >> 1)) >> (shift - 1) : n;
+  }
+};
+
 struct AppendDev {
   Kv8Dev pg;
   const char* x[2];                 // K, V rows
@@ -31,7 +46,9 @@ struct AppendDev {
   const int32_t* counts;
   uint32_t* status;
   int32_t num_tokens;
+  int32_t parts_log2;               // 16-row parts of a page; -1 where they are no power of two
   uint32_t touched, units, all_units;   // touched: pages of a sequence that num_tokens rows can reach; units of a CTA
+  Divisor by_touched, by_heads;
 };
 
 enum NewType { kNewBf16 = 0, kNewF16 = 1, kNewF32 = 2 };
@@ -279,15 +296,16 @@ __global__ void __launch_bounds__(512, !kFew && D <= 128 && NT != kNewF32 ? 2 : 
 
   const int parts = a.pg.page_size >> 4;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int group = warp / (2 * parts), in_group = warp - group * 2 * parts;
+  const int group = a.units == 1 ? 0 : a.parts_log2 >= 0 ? warp >> (a.parts_log2 + 1) : warp / (2 * parts);
+  const int in_group = warp - group * 2 * parts;
   const int kv = in_group >= parts, part = in_group - kv * parts;
   const int bar = 1 + 2 * group + kv;       // a barrier for the warps of each half
   wait_for_previous_grid();
   allow_dependents();
   const uint32_t unit = blockIdx.x * a.units + group;
   if (unit >= a.all_units) return;
-  const uint32_t bh = unit / a.touched, j = unit - bh * a.touched;
-  const int b = (int)(bh / a.pg.heads), h = (int)(bh - b * a.pg.heads);
+  const uint32_t bh = a.by_touched.quotient(unit), j = unit - bh * a.touched;
+  const int b = (int)a.by_heads.quotient(bh), h = (int)(bh - b * a.pg.heads);
 
   // the page and its rows; every exit before the barriers is taken by the whole unit
   const int tok0 = a.tok0[b];
@@ -297,7 +315,7 @@ __global__ void __launch_bounds__(512, !kFew && D <= 128 && NT != kNewF32 ? 2 : 
     if (a.status && lane == 0) atomicOr(a.status, MSKV_STATUS_DST_OOB);
     return;
   }
-  const int p = tok0 / a.pg.page_size + (int)j;
+  const int p = (a.parts_log2 >= 0 ? tok0 >> (a.parts_log2 + 4) : tok0 / a.pg.page_size) + (int)j;
   const int64_t t0 = (int64_t)p * a.pg.page_size;
   const int64_t end = (int64_t)tok0 + n;
   if (t0 >= end) return;
@@ -473,14 +491,18 @@ extern "C" int mskv_kv8_append(const mskv_kv8_append_desc* d, void* stream) {
   a.num_tokens = d->num_tokens;
   a.touched = (uint32_t)(((int64_t)d->num_tokens + a.pg.page_size - 2) / a.pg.page_size + 1);
   const int64_t all = (int64_t)a.touched * a.pg.batch * a.pg.heads;
+  if (all > INT_MAX) return fail(MSKV_ERR_RANGE, "mskv_kv8_append: too many rows for one call");
   a.all_units = (uint32_t)all;
+  a.by_touched = Divisor(a.touched);
+  a.by_heads = Divisor((uint32_t)a.pg.heads);
+  const int parts = a.pg.page_size / 16;
+  a.parts_log2 = parts & (parts - 1) ? -1 : parts >= 8 ? 3 : parts >> 1;
   // Few units: one a CTA and all of a page's rows loaded together; more: up to 8 warps a CTA, in fewer registers.  128 dims,
   // bf16, pages of 16: 32 units 3.4 us against 4.8, 576 units 4.1 against 5.8, 1088 units 7.2 against 6.4, 2176
   // units 14.5 against 8.7.
   const bool few = all <= 4 * (int64_t)sms_of_device();
   a.units = few ? 1 : (uint32_t)std::max(1, 64 / a.pg.page_size);
   const int64_t ctas = (all + a.units - 1) / a.units;
-  if (all > INT_MAX) return fail(MSKV_ERR_RANGE, "mskv_kv8_append: too many rows for one call");
   const bool vec = ((k_bits | v_bits) & 15) == 0;   // 16-byte loads; other layouts element by element
   const bool e5m2 = d->pages.dtype == MSKV_DT_FP8_E5M2;
   const cudaStream_t st = as_stream(stream);
