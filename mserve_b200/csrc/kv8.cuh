@@ -61,6 +61,21 @@ inline int sms_of_device() {
   return n;
 }
 
+// Division by an invariant (Granlund and Montgomery): a multiplication, an average and a shift.
+struct Divisor {
+  uint32_t factor, shift;
+  explicit Divisor(uint32_t d = 1) : factor(1), shift(0) {
+    uint32_t l = 0;
+    while (l < 32 && ((uint64_t)1 << l) < d) ++l;
+    factor = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << l) - d)) / d + 1);
+    shift = l;
+  }
+  __device__ __forceinline__ uint32_t quotient(uint32_t n) const {
+    const uint32_t t = __umulhi(factor, n);
+    return shift ? (t + ((n - t) >> 1)) >> (shift - 1) : n;
+  }
+};
+
 // 2^e for e in [-126, 127].
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 

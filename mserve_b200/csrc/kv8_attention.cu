@@ -71,6 +71,7 @@ struct Kv8AttnDev {
   int32_t cluster, cluster_log2;   // CTAs that share a segment (1, 2, 4, 8); 0: the line
   int32_t parts_log2;              // tiles of a page; -1 where they are no power of two
   int32_t vec_q, pow2_page, aligned;
+  Divisor by_heads;
 };
 
 // Warps of a CTA, its ring's stages and CTAs of an SM, by what the registers (64 dims: 80 a thread, 128 with a second
@@ -837,7 +838,7 @@ kv8_attn_kernel(const Kv8AttnDev a, const __grid_constant__ CUtensorMap k_map, c
       const uint32_t rank = blockIdx.x & (a.cluster - 1), seg = blockIdx.x >> a.cluster_log2;
       const int bh = a.row_tiles == 1 ? (int)seg : (int)(seg / a.row_tiles);
       at.rt = (int)(seg - bh * a.row_tiles);
-      at.b = bh / a.pg.heads;
+      at.b = (int)a.by_heads.quotient(bh);
       at.h = bh - at.b * a.pg.heads;
       at.len = kv8_len(a, at.b);
       at.n = kv8_tiles(a, at.b, at.h);
@@ -905,7 +906,7 @@ __global__ void __launch_bounds__(kKmWarps * 32) kv8_merge_kernel(const Kv8AttnD
   __shared__ __align__(16) float s_o[kKmWarps][D];
   const int seg = blockIdx.x / kRows, r = blockIdx.x % kRows;
   const int rt = seg % a.row_tiles, bh = seg / a.row_tiles;
-  const int b = bh / a.pg.heads, h = bh % a.pg.heads;
+  const int b = (int)a.by_heads.quotient(bh), h = bh - b * a.pg.heads;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // the lengths are those that the first kernel, which waited for whatever wrote them, has read already
   const bool empty = kv8_tiles(a, b, h) == 0;
@@ -1211,6 +1212,7 @@ extern "C" int mskv_kv8_attention(const mskv_kv8_attn_desc* d, void* stream) {
   a.segments = (int32_t)p.segments;
   a.max_tokens = d->max_tokens;
   a.width = d->num_blocks;
+  a.by_heads = Divisor((uint32_t)a.pg.heads);
   a.cluster = p.cluster;
   const int parts = a.pg.page_size / 16;
   a.parts_log2 = parts & (parts - 1) ? -1 : parts >= 8 ? 3 : parts >> 1;

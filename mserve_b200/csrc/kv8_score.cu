@@ -29,6 +29,7 @@ struct BlockScoreDev {
   int64_t stride;
   uint32_t* status;
   int32_t group, max_blocks, chunks, tiles;   // chunks of a (b, h); tiles of 16 blocks a warp takes of one
+  Divisor by_chunks, by_heads;
 };
 
 constexpr int kBsWarps = 8;
@@ -42,8 +43,8 @@ __global__ void __launch_bounds__(kBsWarps * 32, D <= 128 ? 4 : 2) kv8_block_sco
 
   wait_for_previous_grid();
   allow_dependents();
-  const int bh = blockIdx.x / a.chunks, chunk = blockIdx.x - bh * a.chunks;
-  const int b = bh / a.pg.heads, h = bh - b * a.pg.heads;
+  const int bh = (int)a.by_chunks.quotient(blockIdx.x), chunk = (int)blockIdx.x - bh * a.chunks;
+  const int b = (int)a.by_heads.quotient(bh), h = bh - b * a.pg.heads;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int first = chunk * a.tiles * kBsWarps * 16;
   const int j0 = first + warp * 16 + g;
@@ -212,6 +213,8 @@ extern "C" int mskv_kv8_block_score(const mskv_kv8_score_desc* d, void* stream) 
   const int64_t rows = ((int64_t)d->max_blocks + 16 * kBsWarps - 1) / (16 * kBsWarps);
   a.tiles = (int)std::min<int64_t>(4, std::max<int64_t>(1, segs * rows / (2 * sms_of_device())));
   a.chunks = (int)((rows + a.tiles - 1) / a.tiles);
+  a.by_chunks = Divisor((uint32_t)a.chunks);
+  a.by_heads = Divisor((uint32_t)a.pg.heads);
   const int64_t ctas = segs * a.chunks;
   if (ctas > INT_MAX) return fail(MSKV_ERR_RANGE, "mskv_kv8_block_score: too many blocks for one call");
   const bool e5m2 = d->pages.dtype == MSKV_DT_FP8_E5M2, bf16 = d->dtype == MSKV_DT_BF16;
