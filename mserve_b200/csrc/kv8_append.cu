@@ -14,8 +14,8 @@
 //  * Other pages (a decode token joins old rows; fp32 rows) take their rows as fp32, a batch of steps at a time,
 //    a second time from the caches where one batch does not hold them.  Old rows are stored again only
 //    when the exponent changed.
-// Measured: 2 x 16384 bf16 tokens, 8 heads, 128 dims (206 MB) 39 us = 0.80 of the copy rate; 4 x up to 64 fp16 tokens,
-// 8 heads 4.3 us; one token of 8 sequences, 4 heads 3.0 us (launch, length, page id, rows).
+// Measured: 2 x 16384 bf16 tokens, 8 heads, 128 dims (206 MB) 37.4 us = 0.84 of the copy rate; 4 x up to 64 fp16 tokens,
+// 8 heads 4.2 us; one token of 8 sequences, 4 heads 2.8 us (launch, length, page id, rows).
 #include <algorithm>
 #include <type_traits>
 

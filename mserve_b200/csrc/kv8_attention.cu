@@ -34,7 +34,7 @@
 // lengths in every CTA); a segment of several parts goes through the workspace and a second kernel.
 //
 // Measured (device time, three sets of inputs in turn): 40/8 heads, 128 dims, 16 sequences of 32768 tokens
-// (1.07 GB) 172 us = 0.95 of the copy rate; 28/4 heads, 8 of 16384 (134 MB) 27.6 us = 0.75, of which 3 us pass
+// (1.07 GB) 173 us = 0.95 of the copy rate; 28/4 heads, 8 of 16384 (134 MB) 28.6 us = 0.72, of which 3 us pass
 // before the first codes are there and 2 after the last; 136 listed pages of each (18 MB) 8.8 us.
 // Loads straight into registers instead of the ring (one tile ahead, as many as the registers hold): 181,
 // 32.5 and 11.7 us, and 10% more than that at the clocks of a GPU at its power limit; the same chunks through

@@ -12,8 +12,8 @@
 // both columns' sums.  FMAs in fp32 would need an unpacking and an FMA per code and a
 // shuffle reduction; the tensor core needs neither.  The next tile's page ids are looked up during a tile, its
 // bounds loaded as soon as the tile's are in the products.
-// Measured: 56/8 heads, 128 dims, 16 sequences of up to 65536 tokens in pages of 16 (77 MB) 16.4 us = 0.72 of the copy
-// rate; 28/4 heads, 8 of 16384 (8.6 MB) 4.9 us, a chain of launch, page id, bounds and products.
+// Measured: 56/8 heads, 128 dims, 16 sequences of up to 65536 tokens in pages of 16 (77 MB) 16.0 to 16.8 us = 0.72 of the
+// copy rate; 28/4 heads, 8 of 16384 (8.6 MB) 4.8 us, a chain of launch, page id, bounds and products.
 #include <algorithm>
 
 #include "kv8.cuh"
@@ -207,7 +207,7 @@ extern "C" int mskv_kv8_block_score(const mskv_kv8_score_desc* d, void* stream) 
   a.group = d->q_heads / d->pages.kv_heads;
   a.max_blocks = d->max_blocks;
   // Tiles a warp takes per CTA: one while that fits one wave of the GPU, up to four beyond, so that the weights' set-up is
-  // shared.  One, two, four, eight: 8 sequences of 1024 pages, 4 heads 4.9, 5.8, 7.7, 11.3 us; 16 of 2048, 8 heads
+  // shared.  One, two, four, eight: 8 sequences of 1024 pages, 4 heads 4.8, 5.8, 7.7, 11.3 us; 16 of 2048, 8 heads
   // 20.0, 16.6, 14.7, 15.5 us; 64 of 256, 4 heads 6.8, 7.2, 7.2, 7.3 us.
   const int64_t segs = (int64_t)a.pg.batch * a.pg.heads;
   const int64_t rows = ((int64_t)d->max_blocks + 16 * kBsWarps - 1) / (16 * kBsWarps);

@@ -90,7 +90,10 @@ class PagedKV8:
         self.len_h = new_len
 
     def reset(self, b: int) -> None:
-        """Empties sequence b: its pages are free for others from the next step on."""
+        """Empties sequence b: its pages are free for others from the next step on.
+
+        Called between steps: a step that is under way loses the rows it has not appended yet.
+        """
         if not 0 <= b < self.B:
             raise ValueError(f"no sequence {b}")
         row = self.page_table_h[b]
