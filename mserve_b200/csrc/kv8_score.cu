@@ -12,7 +12,7 @@
 // both columns' sums.  FMAs in fp32 would need an unpacking and an FMA per code and a
 // shuffle reduction; the tensor core needs neither.  The next tile's page ids are looked up during a tile, its
 // bounds loaded as soon as the tile's are in the products.
-// Measured: 56/8 heads, 128 dims, 16 sequences of up to 65536 tokens in pages of 16 (77 MB) 16.0 to 16.8 us = 0.72 of the
+// Measured: 56/8 heads, 128 dims, 16 sequences of up to 65536 tokens in pages of 16 (77 MB) 16.0 us = 0.74 of the
 // copy rate; 28/4 heads, 8 of 16384 (8.6 MB) 4.8 us, a chain of launch, page id, bounds and products.
 #include <algorithm>
 
