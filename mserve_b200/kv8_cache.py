@@ -118,7 +118,10 @@ class PagedKV8:
 
     # ------------------------------------------------------------------ a layer of the step
     def append_layer(self, layer: int, k_new: torch.Tensor, v_new: torch.Tensor) -> None:
-        """The step's rows [B, Hkv, n, D] of one layer (n at least every sequence's n_new; fp32, fp16 or bf16)."""
+        """The step's rows [B, Hkv, n, D] of one layer (n at least every sequence's n_new; fp32, fp16 or bf16).
+
+        A captured call writes n rows at most: its replays are for steps of up to n tokens.
+        """
         if k_new.dim() != 4 or k_new.shape[:2] != (self.B, self.Hkv) or k_new.shape[3] != self.D:
             raise ValueError(f"k_new must be [B={self.B}, Hkv={self.Hkv}, n, D={self.D}]")
         if k_new.shape[2] < int(self._stage[1].max()):
