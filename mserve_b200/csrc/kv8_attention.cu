@@ -1073,7 +1073,12 @@ static Kv8Plan make_plan(const mskv_kv8_attn_desc& d) {
   const double alone_us = tile_us * ((most + warps * cluster - 1) / (warps * cluster));
   const double fill = (double)p.segments * cluster / slots;
   const double line_us = fill * (d.blocks ? codes_us : std::min(0.85 * codes_us, 25.0)) + (p.segments * 2 > slots ? 8 : 4);
-  if (most <= 4 * warps * cluster || (fill <= 1 && alone_us <= line_us)) {
+  // Of several waves of segments, each is a CTA's own while the longest takes no longer than the starts that a CTA of
+  // the line has for all of its segments, 8 us each.  Own / line, ragged, 5 positions: 96/8 heads of 64 dims, 43 lists
+  // of up to 504 tokens 40 / 127 us; 56/8 heads, 30 of up to 997 54 / 150; of 256 dims, 96/8 heads, 28 of up to 1100 130 / 259;
+  // 64/8 heads, 4 positions, 64 of up to 8192 268 / 350.
+  const bool many = p.segments > slots && alone_us <= 8.0 * fill;
+  if (most <= 4 * warps * cluster || many || (fill <= 1 && alone_us <= line_us)) {
     p.cluster = cluster;
     p.ctas = p.segments * cluster;
     return p;
