@@ -29,7 +29,7 @@
 // the legacy pipe is a fifth busy at the memory's speed.
 //
 // Split: a segment is a (sequence, KV head, row tile).  Where the segments fill the GPU evenly, or are short, a
-// thread-block cluster takes each and merges through distributed shared memory.  Otherwise all tiles of all
+// thread-block cluster (of one CTA, where they are many) takes each and merges through distributed shared memory.  Otherwise all tiles of all
 // segments form one line, cut into parts for the CTAs however ragged the lengths are (a scan over the
 // lengths in every CTA); a segment of several parts goes through the workspace and a second kernel.
 //

@@ -423,6 +423,23 @@ def test_many_ragged_sequences(built_lib):
     _close(out, want, bound)
 
 
+@pytest.mark.parametrize("B,H,G,D,Q,most,qt", [(80, 4, 7, 128, 1, 700, torch.bfloat16), (60, 4, 7, 128, 5, 900, torch.float16),
+                                               (40, 3, 5, 256, 5, 700, torch.bfloat16), (30, 4, 12, 64, 5, 600, torch.float16)])
+def test_several_waves_of_segments(built_lib, B, H, G, D, Q, most, qt):
+    """More segments than CTAs at once, short ones: a CTA takes each from its first to its last token."""
+    from mserve_b200 import ops
+    g = torch.Generator().manual_seed(D + Q)
+    lens = torch.randint(0, most + 1, (B,), generator=g).tolist()
+    lens[0], lens[1], lens[-1] = most, 0, 1
+    pages, table, g = _filled(B, H, D, 32, E4M3, lens, seed=D)
+    q = (torch.randn(B, H * G, Q, D, generator=g) * 0.5).to(qt)
+    out = torch.full(q.shape, float("nan"), dtype=qt, device="cuda")
+    ops.kv8_attention(q.cuda(), pages, table.cuda(), lens=_i32(lens), max_tokens=most, out=out)
+    ops.check_status(torch.device("cuda"))
+    want, bound = k8.attention(q.double(), _host(pages), table, lens, weight_bits=_bits(qt))
+    _close(out, want, bound)
+
+
 def test_large_offsets(built_lib):
     """Pools past 2^31 bytes, with the sequence's pages at both ends."""
     from mserve_b200 import ops
