@@ -47,7 +47,7 @@ extern "C" {
 #define MSKV_STATUS_INDEX_OOB 0x1u   /* a source token index was outside [0, len)            */
 #define MSKV_STATUS_BAD_PAGE 0x2u    /* a page-table entry needed by a row was negative      */
 #define MSKV_STATUS_DST_OOB 0x4u     /* a destination token was outside [0, len)             */
-#define MSKV_STATUS_TIMEOUT 0x8u     /* a bounded wait (mskv_flag_wait) reached its time limit */
+#define MSKV_STATUS_TIMEOUT 0x8u     /* a bounded wait (a load, mskv_flag_wait) reached its limit */
 
 /* ---- element types ---------------------------------------------------------------------- */
 #define MSKV_DT_F32 0
@@ -457,7 +457,8 @@ int mskv_kv8_block_score(const mskv_kv8_score_desc* d, void* stream);
  * outputs).  `workspace` must hold mskv_kv8_attention_workspace_bytes(d) bytes of device memory,
  * 16-byte aligned; every launch writes all it reads of it.  Calls that may overlap must not share one.
  * stride_page and stride_h must lie in (0, 2^40) here (codes are loaded by TMA).  Every wait on such a load
- * is bounded; one that runs out leaves the row incomplete and sets MSKV_STATUS_TIMEOUT.
+ * is bounded; one that runs out leaves the row incomplete and sets MSKV_STATUS_TIMEOUT (the block that
+ * waited drops its share of its rows, waits, bounded again, for its other loads and takes no further ones).
  * q (b, hq, i, d) at q + b*q_stride_b + hq*q_stride_h + i*q_stride_q (bytes) + d elements, out
  * likewise.                                                                                 */
 typedef struct mskv_kv8_attn_desc {
@@ -487,6 +488,10 @@ typedef struct mskv_kv8_attn_desc {
 } mskv_kv8_attn_desc;
 uint64_t mskv_kv8_attention_workspace_bytes(const mskv_kv8_attn_desc* d);
 int mskv_kv8_attention(const mskv_kv8_attn_desc* d, void* stream);
+/* Non-zero: in the mskv_kv8_attention calls that follow, the first wait for a load of every part of the work counts
+ * as expired, so that a caller's handling of MSKV_STATUS_TIMEOUT can be tried without a fault; zero, the
+ * default: not.  For the whole process.  Returns the value before.                          */
+int32_t mskv_kv8_expire_waits(int32_t on);
 
 /* ---- peer memory and flags (score-row exchange between the GPUs of one node) --------------
  * The shared selection's exchange of score rows (attention.py:558-572 with the KV heads on

@@ -175,6 +175,7 @@ SIGNATURES = [
     ("mskv_kv8_block_score", C.c_int, [C.POINTER(Kv8ScoreDesc), _vp]),
     ("mskv_kv8_attention_workspace_bytes", C.c_uint64, [C.POINTER(Kv8AttnDesc)]),
     ("mskv_kv8_attention", C.c_int, [C.POINTER(Kv8AttnDesc), _vp]),
+    ("mskv_kv8_expire_waits", _i32, [_i32]),
     ("mskv_ipc_handle_bytes", C.c_uint64, []),
     ("mskv_ipc_alloc", C.c_int, [C.c_uint64, C.POINTER(_vp), _vp]),
     ("mskv_ipc_open", C.c_int, [_vp, C.POINTER(_vp)]),

@@ -46,6 +46,7 @@
 #include <atomic>
 
 #include "kv8.cuh"
+#include "ring.cuh"
 #include "tensor_map.cuh"
 
 namespace cg = cooperative_groups;
@@ -71,6 +72,7 @@ struct Kv8AttnDev {
   int32_t cluster, cluster_log2;   // CTAs that share a segment (1, 2, 4, 8); 0: the line
   int32_t parts_log2;              // tiles of a page; -1 where they are no power of two
   int32_t vec_q, pow2_page, aligned;
+  int32_t expire;                  // every first wait for codes counts as expired (mskv_kv8_expire_waits)
   Divisor by_heads;
 };
 
@@ -162,6 +164,7 @@ struct Kv8Attn {
     __half q[kRows][D + 8];
     float f[kRows];
     int lim[kRows];                               // tokens that a row sees
+    uint32_t expired;                             // a wait of one of the warps ran out
   };
 
   // With two column tiles the query's fragments stay in shared memory (the registers hold O and the codes).
@@ -555,23 +558,35 @@ struct Kv8Attn {
     const int len = at.len;
     const int seen_by_all = len - a.q_len + 1;    // tokens below: every row sees them
     const int mine = first + warp;
-    const int n = mine < last ? (last - mine + kWarps - 1) / kWarps : 0;
+    int n = mine < last ? (last - mine + kWarps - 1) / kWarps : 0;
     // lane j describes this warp's tile 32*k + j; the next 32 are looked up halfway through
     Tile now{-1, 0, 0}, next{-1, 0, 0};
     if (lane < n) now = find(a, b, h, len, mine + lane * kWarps);
     const QRows q = load_q(a, b, h, rt, warp, lane);
     const uint32_t ring = smem_addr(&sm.ring[warp][0][0]), bars = smem_addr(&sm.arrived[warp][0]);
-    int stage = (int)(turn % kStages);            // of tile i; tile number turn + i of the warp
+    RingPlace<kStages> place(turn);               // of tile i; tile number turn + i of the warp
 #pragma unroll 1
     for (int i = 0; i < kStages; ++i) {
       const int page = __shfl_sync(0xffffffffu, now.page, i), tok = __shfl_sync(0xffffffffu, now.tok, i);
-      const int to = stage + i < kStages ? stage + i : stage + i - kStages;
+      const int to = place.stage_ahead(i);
       if (lane == 0 && i < n) fetch(a, k_map, v_map, page, tok, h, ring + to * kTileBytes, bars + 8 * to);
     }
     stage_q(a, sm, q, rt, len, warp, lane);
     __syncthreads();
     start(sm, lane);
-    uint32_t phase = (turn / kStages) & 1;
+    // The bounded wait for tile i ran out: the rows are incomplete, so say so, wait (again with a limit) for the copies
+    // still in flight and take no more tiles, of this segment or another: the CTA contributes nothing from here on.
+    const auto give_up = [&](int i) {
+      if (lane == 0) {
+        if (a.status) atomicOr(a.status, MSKV_STATUS_TIMEOUT);
+        sm.expired = 1;
+      }
+      place.drain(i, n, [&](int stage, uint32_t phase) { return bulk_wait(bars + 8 * stage, phase); });
+    };
+    if (a.expire && n > 0) {
+      give_up(0);
+      n = 0;
+    }
 #pragma unroll 1
     for (int i = 0; i < n; ++i) {
       if ((i & 31) == 16) {
@@ -580,12 +595,9 @@ struct Kv8Attn {
         if (j < n) next = find(a, at.b, h, len, (int)(at.at - at.start) + warp + j * kWarps);
       }
       const int tok = __shfl_sync(0xffffffffu, now.tok, i & 31), exps = __shfl_sync(0xffffffffu, now.exps, i & 31);
-      const uint32_t tile = ring + stage * kTileBytes;
-      if (!__all_sync(0xffffffffu, bulk_wait(bars + 8 * stage, phase))) {
-        // The bounded wait ran out: the rows are incomplete, so say so and take no more tiles; the copies still
-        // in flight are waited for (again with a limit) before their memory is used otherwise.
-        if (lane == 0 && a.status) atomicOr(a.status, MSKV_STATUS_TIMEOUT);
-        for (int k = 0; k < kStages; ++k) bulk_wait(bars + 8 * k, phase);
+      const uint32_t bar = bars + 8 * place.stage, tile = ring + place.stage * kTileBytes;
+      if (!__all_sync(0xffffffffu, bulk_wait(bar, place.phase))) {
+        give_up(i);
         break;
       }
       if (exps & 0x10000) {
@@ -601,18 +613,16 @@ struct Kv8Attn {
       const bool other = (i & 31) + kStages > 31;
       const int page_ahead = __shfl_sync(0xffffffffu, other ? next.page : now.page, (i + kStages) & 31);
       const int tok_ahead = __shfl_sync(0xffffffffu, other ? next.tok : now.tok, (i + kStages) & 31);
-      if (lane == 0 && i + kStages < n) fetch(a, k_map, v_map, page_ahead, tok_ahead, h, tile, bars + 8 * stage);
-      if (++stage == kStages) {
-        stage = 0;
-        phase ^= 1;
-      }
+      if (lane == 0 && i + kStages < n) fetch(a, k_map, v_map, page_ahead, tok_ahead, h, tile, bar);
+      place.advance();
       if ((i & 31) == 31) now = next;
     }
     turn += n;
     collect(sm, warp, lane);
   }
 
-  // The warps' (m, l, O) to shared memory, O relative to the CTA's m.
+  // The warps' (m, l, O) to shared memory, O relative to the CTA's m.  O takes the ring's place, so not after an
+  // expired wait, when a copy may still be under way to it.
   __device__ __forceinline__ void collect(Smem& sm, int warp, int lane) {
     const int g = lane >> 2, c = lane & 3;
 #pragma unroll
@@ -629,6 +639,7 @@ struct Kv8Attn {
         }
       }
     __syncthreads();
+    if (sm.expired) return;                       // the whole CTA
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -650,12 +661,13 @@ struct Kv8Attn {
     __syncthreads();
   }
 
-  // Sums of the CTA for dims d .. d+3 of row r, after collect.
+  // Sums of the CTA for dims d .. d+3 of row r, after collect; nothing after an expired wait.
   struct Part {
     float4 x;
     float top, sum;
   };
-  static __device__ __forceinline__ Part cta_part(const Smem& sm, int r, int d) {
+  static __device__ __forceinline__ Part cta_part(const Smem& sm, bool expired, int r, int d) {
+    if (expired) return {make_float4(0.f, 0.f, 0.f, 0.f), kNoMax, 0.f};
     Part y{make_float4(0.f, 0.f, 0.f, 0.f), sm.m[0][r], 0.f};
 #pragma unroll
     for (int w = 1; w < kWarps; ++w) y.top = fmaxf(y.top, sm.m[w][r]);
@@ -670,10 +682,11 @@ struct Kv8Attn {
 
   // Writes the CTA's rows after a piece: to `out`, or (slot >= 0) to the workspace.
   static __device__ __forceinline__ void finish(const Kv8AttnDev& a, const Smem& sm, const Place& at, int slot) {
+    const bool expired = sm.expired;
 #pragma unroll 1
     for (int i = threadIdx.x; i < kRows * D / 4; i += kThreads) {
       const int r = i / (D / 4), d = (i % (D / 4)) * 4;
-      const Part y = cta_part(sm, r, d);
+      const Part y = cta_part(sm, expired, r, d);
       if (slot >= 0) {
         *reinterpret_cast<float4*>(a.part_o + ((int64_t)slot * kRows + r) * D + d) = y.x;
         if (d == 0) *reinterpret_cast<float2*>(a.part_ml + ((int64_t)slot * kRows + r) * 2) = make_float2(y.top, y.sum);
@@ -687,12 +700,13 @@ struct Kv8Attn {
   // memory of CTA r % ctas, which finishes the row after one barrier of the cluster (nothing reads another
   // CTA's memory after that, so each may end).
   static __device__ __forceinline__ void finish_cluster(const Kv8AttnDev& a, Smem& sm, const Place& at, int rank, int ctas, int log2) {
+    const bool expired = sm.expired;
     cg::cluster_group cluster = cg::this_cluster();
     cluster.barrier_wait();                       // all CTAs of the cluster run (they arrived when they began)
 #pragma unroll 1
     for (int i = threadIdx.x; i < kRows * D / 4; i += kThreads) {
       const int r = i / (D / 4), d = (i % (D / 4)) * 4, owner = r & (ctas - 1), slot = rank * (kRows >> log2) + (r >> log2);
-      const Part y = cta_part(sm, r, d);
+      const Part y = cta_part(sm, expired, r, d);
       *cluster.map_shared_rank(reinterpret_cast<float4*>(&sm.sent[slot][d]), owner) = y.x;
       if (d == 0) *cluster.map_shared_rank(&sm.sent_ml[slot], owner) = make_float2(y.top, y.sum);
     }
@@ -823,6 +837,7 @@ kv8_attn_kernel(const Kv8AttnDev a, const __grid_constant__ CUtensorMap k_map, c
   if (threadIdx.x == 0) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
+    sm.expired = 0;
   }
   if (a.cluster > 1) cg::this_cluster().barrier_arrive();
   if (lane == 0) {
@@ -858,7 +873,7 @@ kv8_attn_kernel(const Kv8AttnDev a, const __grid_constant__ CUtensorMap k_map, c
   K k;
   uint32_t turn = 0;               // tiles that this warp has taken
   for (;;) {
-    k.piece(a, &k_map, &v_map, sm, at, turn, warp, lane);
+    if (!sm.expired) k.piece(a, &k_map, &v_map, sm, at, turn, warp, lane);   // stable here: set before a piece's last barrier
     if (a.cluster > 1) {
       K::finish_cluster(a, sm, at, (int)(blockIdx.x & (a.cluster - 1)), a.cluster, a.cluster_log2);
       return;
@@ -1097,6 +1112,8 @@ static Kv8Plan make_plan(const mskv_kv8_attn_desc& d) {
   return p;
 }
 
+static std::atomic<int32_t> g_expire{0};   // mskv_kv8_expire_waits
+
 // K or V as a 4-D tensor [page][head][row][dim] of bytes, in boxes of 16 rows and at most 128 dims.
 static bool encode_pages_map(CUtensorMap* m, uint8_t* base, const Kv8Dev& pg, int d) {
   const EncodeTiledFn encode = tensor_map_encoder();
@@ -1184,6 +1201,8 @@ extern "C" uint64_t mskv_kv8_attention_workspace_bytes(const mskv_kv8_attn_desc*
   return p.info_bytes + p.ml_bytes + p.o_bytes;
 }
 
+extern "C" int32_t mskv_kv8_expire_waits(int32_t on) { return g_expire.exchange(on != 0, std::memory_order_relaxed); }
+
 extern "C" int mskv_kv8_attention(const mskv_kv8_attn_desc* d, void* stream) {
   if (const int rc = check_attn(d)) return rc;
   if (!d->q || !d->out || !d->lens) return fail(MSKV_ERR_ARG, "mskv_kv8_attention: NULL q, out or lens");
@@ -1225,6 +1244,7 @@ extern "C" int mskv_kv8_attention(const mskv_kv8_attn_desc* d, void* stream) {
   a.aligned = p.aligned;
   a.vec_q = (q_bits & 15) == 0;
   a.pow2_page = (a.pg.page_size & (a.pg.page_size - 1)) == 0;
+  a.expire = g_expire.load(std::memory_order_relaxed);
   const bool e5m2 = d->pages.dtype == MSKV_DT_FP8_E5M2, bf16 = d->dtype == MSKV_DT_BF16;
   const cudaStream_t st = as_stream(stream);
   switch (d->pages.head_dim) {

@@ -80,7 +80,7 @@ def describe_status(v: int) -> str:
     if v & _lib.STATUS_DST_OOB:
         reasons.append("destination token out of range")
     if v & _lib.STATUS_TIMEOUT:
-        reasons.append("a wait for another GPU's flag timed out")
+        reasons.append("a bounded wait (a load, or another GPU's flag) timed out")
     return f"{', '.join(reasons)} (status 0x{v:x})"
 
 
