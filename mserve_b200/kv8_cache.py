@@ -132,8 +132,9 @@ class PagedKV8:
         """Pages for q's last position: (indices [B, Hkv, top + recent], ascending, counts [B, Hkv])."""
         ops.kv8_block_score(q, self.pages[layer], self.page_table, lens=self.lens, max_blocks=self.max_pages,
                             out=self._scores)
-        ops.topk(self._scores.view(self.B * self.Hkv, self.max_pages), top_k=self.top_blocks, recent=self.recent_blocks,
-                 len_=self.held, len_scalar=self.max_pages, sel_per_batch=self.Hkv, out=self._idx, counts=self._counts)
+        with torch.cuda.device(self.device):        # ops.topk launches on the current device
+            ops.topk(self._scores.view(self.B * self.Hkv, self.max_pages), top_k=self.top_blocks, recent=self.recent_blocks,
+                     len_=self.held, len_scalar=self.max_pages, sel_per_batch=self.Hkv, out=self._idx, counts=self._counts)
         return self._idx.view(self.B, self.Hkv, -1), self._counts.view(self.B, self.Hkv)
 
     def decode_layer(self, layer: int, q: torch.Tensor, *, out: Optional[torch.Tensor] = None,

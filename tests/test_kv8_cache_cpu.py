@@ -1,0 +1,51 @@
+"""PagedKV8's host side without a GPU: the calls that a step makes, on stand-ins for the operators."""
+import contextlib
+
+import numpy as np
+import pytest
+import torch
+
+
+@pytest.fixture
+def engine(monkeypatch, built_lib):
+    """make(...): a PagedKV8 on CPU tensors whose operator calls are recorded in make.calls as (name, device that is
+    current, arguments)."""
+    from mserve_b200 import kv8_cache, ops
+    calls, current = [], [None]
+
+    @contextlib.contextmanager
+    def on(device):
+        was, current[0] = current[0], device
+        yield
+        current[0] = was
+
+    def record(name, result=None):
+        def call(*args, **kw):
+            calls.append((name, current[0], args, kw))
+            return result(*args, **kw) if result else None
+        return call
+
+    def topk(scores, *, top_k, recent=0, out=None, counts=None, **kw):
+        n = scores.shape[0]
+        return (torch.zeros(n, top_k + recent, dtype=torch.int32) if out is None else out,
+                torch.zeros(n, dtype=torch.int32) if counts is None else counts)
+
+    monkeypatch.setattr(torch.cuda, "device", on)
+    monkeypatch.setattr(torch.Tensor, "pin_memory", lambda t, *a: t)
+    monkeypatch.setattr(ops, "kv8_append", record("append"))
+    monkeypatch.setattr(ops, "kv8_block_score", record("score"))
+    monkeypatch.setattr(ops, "topk", record("topk", topk))
+    monkeypatch.setattr(ops, "kv8_attention", record("attention", lambda q, *a, **kw: torch.zeros_like(q)))
+
+    def make(*args, **kw):
+        return kv8_cache.PagedKV8(*args, device=torch.device("cpu"), **kw)
+    make.calls = calls
+    return make
+
+
+def test_selection_runs_on_the_caches_device(engine):
+    """The top-k call, which launches on the current device, is made with the cache's device current."""
+    eng = engine(1, 2, 4, 2, 64, 100, top_blocks=2)
+    eng.decode_layer(0, torch.zeros(2, 4, 64, dtype=torch.bfloat16))
+    assert [c[0] for c in engine.calls] == ["score", "topk", "attention"]
+    assert engine.calls[1][1] == eng.device
