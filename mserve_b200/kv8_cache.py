@@ -7,7 +7,7 @@ power-of-two scale per (page, KV head) and the pages' key bounds (ops.Kv8Pages),
 
 A decode step, per layer: the step's tokens are appended (mskv_kv8_append), then either the whole cache is
 attended (mskv_kv8_attention) or, with ``top_blocks``, every page is scored from its bounds
-(mskv_kv8_block_score), the best pages and the last ``recent_blocks`` are selected per (sequence, KV head)
+(mskv_kv8_block_score), the best pages and the last ones are selected per (sequence, KV head)
 (mskv_topk) and attention runs over those.  No host synchronisation: ``begin_step`` sends the step's
 lengths through pinned staging, so the per-layer calls can be captured once in a CUDA graph and replayed
 while the cache grows.
@@ -27,8 +27,8 @@ class PagedKV8:
 
     q_heads, kv_heads, head_dim: the model's (this rank's share, when heads are sharded); page_size: tokens
     per page; cache_dtype: torch.float8_e4m3fn or torch.float8_e5m2.  top_blocks > 0: attention over the
-    top_blocks best pages and the last recent_blocks (at least 1: the step's own tokens) of
-    every (sequence, KV head); 0: over the whole cache.
+    top_blocks best pages and the last recent_blocks (at least 1) of every (sequence, KV head), the pages of
+    the query's own positions always among the last; 0: over the whole cache.
     """
 
     def __init__(self, num_layers: int, batch: int, q_heads: int, kv_heads: int, head_dim: int, capacity: int, *,
@@ -62,7 +62,8 @@ class PagedKV8:
         self._stage_ev: Optional[torch.cuda.Event] = None
         if top_blocks:
             self._scores = torch.empty(batch, kv_heads, self.max_pages, dtype=torch.float32, device=self.device)
-            self._idx = torch.empty(batch * kv_heads, top_blocks + recent_blocks, dtype=torch.int32, device=self.device)
+            self._idx = torch.empty(batch * kv_heads, top_blocks + self._recent(ops.KV8_MAX_POSITIONS), dtype=torch.int32,
+                                    device=self.device)
             self._counts = torch.empty(batch * kv_heads, dtype=torch.int32, device=self.device)
 
     # ------------------------------------------------------------------ lengths and pages
@@ -128,12 +129,21 @@ class PagedKV8:
             raise ValueError(f"the step appends up to {int(self._stage[1].max())} tokens, k_new holds {k_new.shape[2]}")
         ops.kv8_append(self.pages[layer], self.page_table, k_new, v_new, tok0=self.tok0, counts=self.n_new)
 
+    def _recent(self, positions: int) -> int:
+        """Last pages that are always attended: recent_blocks, and those of the last `positions` tokens wherever they end in a page."""
+        return max(self.recent_blocks, 1 - (1 - positions) // self.page_size)
+
     def select(self, layer: int, q: torch.Tensor):
-        """Pages for q's last position: (indices [B, Hkv, top + recent], ascending, counts [B, Hkv])."""
+        """Pages for q [B, Hq, D] or [B, Hq, Q, D]: (indices [B, Hkv, >= top + recent], ascending, counts [B, Hkv]).
+
+        The best top_blocks are those of the last position's scores; the last pages are recent_blocks, or as many as the Q
+        positions' own tokens can lie in (two, where Q > 1) if that is more, so every position attends to itself.
+        """
+        recent = self._recent(q.shape[2] if q.dim() == 4 else 1)
         ops.kv8_block_score(q, self.pages[layer], self.page_table, lens=self.lens, max_blocks=self.max_pages,
                             out=self._scores)
         with torch.cuda.device(self.device):        # ops.topk launches on the current device
-            ops.topk(self._scores.view(self.B * self.Hkv, self.max_pages), top_k=self.top_blocks, recent=self.recent_blocks,
+            ops.topk(self._scores.view(self.B * self.Hkv, self.max_pages), top_k=self.top_blocks, recent=recent,
                      len_=self.held, len_scalar=self.max_pages, sel_per_batch=self.Hkv, out=self._idx, counts=self._counts)
         return self._idx.view(self.B, self.Hkv, -1), self._counts.view(self.B, self.Hkv)
 

@@ -49,3 +49,22 @@ def test_selection_runs_on_the_caches_device(engine):
     eng.decode_layer(0, torch.zeros(2, 4, 64, dtype=torch.bfloat16))
     assert [c[0] for c in engine.calls] == ["score", "topk", "attention"]
     assert engine.calls[1][1] == eng.device
+
+
+@pytest.mark.parametrize("page", [16, 32, 128])
+@pytest.mark.parametrize("recent", [1, 2, 5])
+def test_recent_window_holds_the_positions_own_pages(engine, page, recent):
+    """Whatever the length: the pages of the last Q tokens are among the last pages that the selection always takes."""
+    eng = engine(1, 2, 4, 2, 64, 1000, top_blocks=3, recent_blocks=recent, page_size=page)
+    for Q in (1, 2, 3, 4, 15, 16):
+        engine.calls.clear()
+        q = torch.zeros(2, 4, Q, 64, dtype=torch.bfloat16)
+        eng.decode_layer(0, q)
+        window = next(c[3]["recent"] for c in engine.calls if c[0] == "topk")
+        assert window >= recent and (Q > 1 or window == recent)
+        for n in range(Q, 3 * page + 20):
+            assert (n - 1) // page - (n - Q) // page < window, (Q, n)
+        assert window == recent or any((n - 1) // page - (n - Q) // page == window - 1 for n in range(Q, 3 * page)), "wider than needed"
+    engine.calls.clear()
+    eng.decode_layer(0, torch.zeros(2, 4, 64, dtype=torch.bfloat16))
+    assert next(c[3]["recent"] for c in engine.calls if c[0] == "topk") == recent
