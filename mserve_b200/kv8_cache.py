@@ -60,11 +60,7 @@ class PagedKV8:
         self._stage = torch.zeros(4, batch, dtype=torch.int32).pin_memory()
         self._pt_stage = torch.empty(batch, self.max_pages, dtype=torch.int32).pin_memory()
         self._stage_ev: Optional[torch.cuda.Event] = None
-        if top_blocks:
-            self._scores = torch.empty(batch, kv_heads, self.max_pages, dtype=torch.float32, device=self.device)
-            self._idx = torch.empty(batch * kv_heads, top_blocks + self._recent(ops.KV8_MAX_POSITIONS), dtype=torch.int32,
-                                    device=self.device)
-            self._counts = torch.empty(batch * kv_heads, dtype=torch.int32, device=self.device)
+        self._idx = self._counts = None             # of the last selection, for inspection
 
     # ------------------------------------------------------------------ lengths and pages
     def begin_step(self, n_new: Union[int, Sequence[int]] = 1) -> None:
@@ -134,17 +130,18 @@ class PagedKV8:
         return max(self.recent_blocks, 1 - (1 - positions) // self.page_size)
 
     def select(self, layer: int, q: torch.Tensor):
-        """Pages for q [B, Hq, D] or [B, Hq, Q, D]: (indices [B, Hkv, >= top + recent], ascending, counts [B, Hkv]).
+        """Pages for q [B, Hq, D] or [B, Hq, Q, D]: (indices [B, Hkv, top + recent], ascending, counts [B, Hkv]), the caller's own.
 
         The best top_blocks are those of the last position's scores; the last pages are recent_blocks, or as many as the Q
         positions' own tokens can lie in (two, where Q > 1) if that is more, so every position attends to itself.
         """
         recent = self._recent(q.shape[2] if q.dim() == 4 else 1)
-        ops.kv8_block_score(q, self.pages[layer], self.page_table, lens=self.lens, max_blocks=self.max_pages,
-                            out=self._scores)
+        scores = torch.empty(self.B, self.Hkv, self.max_pages, dtype=torch.float32, device=self.device)
+        ops.kv8_block_score(q, self.pages[layer], self.page_table, lens=self.lens, max_blocks=self.max_pages, out=scores)
         with torch.cuda.device(self.device):        # ops.topk launches on the current device
-            ops.topk(self._scores.view(self.B * self.Hkv, self.max_pages), top_k=self.top_blocks, recent=recent,
-                     len_=self.held, len_scalar=self.max_pages, sel_per_batch=self.Hkv, out=self._idx, counts=self._counts)
+            self._idx, self._counts = ops.topk(scores.view(self.B * self.Hkv, self.max_pages), top_k=self.top_blocks,
+                                               recent=recent, len_=self.held, len_scalar=self.max_pages,
+                                               sel_per_batch=self.Hkv)
         return self._idx.view(self.B, self.Hkv, -1), self._counts.view(self.B, self.Hkv)
 
     def decode_layer(self, layer: int, q: torch.Tensor, *, out: Optional[torch.Tensor] = None,

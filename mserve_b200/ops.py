@@ -544,7 +544,6 @@ def image_filter(attn0: torch.Tensor, *, img_start: int, img_seq: int, text_star
 # 8-bit paged KV cache: append, block scores, attention (whole or over selected blocks)
 # ---------------------------------------------------------------------------------------
 KV8_DTYPES = (torch.float8_e4m3fn, torch.float8_e5m2)
-KV8_MAX_POSITIONS = _lib.KV8_MAX_QLEN       # query positions of a kv8_attention call
 
 
 class Kv8Pages(NamedTuple):

@@ -68,3 +68,15 @@ def test_recent_window_holds_the_positions_own_pages(engine, page, recent):
     engine.calls.clear()
     eng.decode_layer(0, torch.zeros(2, 4, 64, dtype=torch.bfloat16))
     assert next(c[3]["recent"] for c in engine.calls if c[0] == "topk") == recent
+
+
+def test_selections_share_nothing(engine):
+    """Scores, indices and counts of two selections, of one layer or two, are memory of their own."""
+    eng = engine(2, 2, 4, 2, 64, 1000, top_blocks=3)
+    q = torch.zeros(2, 4, 64, dtype=torch.bfloat16)
+    held = [eng.select(layer, q) for layer in (0, 1, 0)]
+    scores = [c[3]["out"] for c in engine.calls if c[0] == "score"]
+    for tensors in (scores, [s[0] for s in held], [s[1] for s in held]):
+        assert len({t.data_ptr() for t in tensors}) == 3
+    assert [c[2][0].data_ptr() for c in engine.calls if c[0] == "topk"] == [t.data_ptr() for t in scores]
+    assert held[0][0].shape == (2, 2, 4) and held[0][1].shape == (2, 2)

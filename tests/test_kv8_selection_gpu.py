@@ -41,3 +41,34 @@ def test_positions_attend_to_themselves(built_lib, page, lens, Q):
                                weight_bits=_bits(torch.bfloat16))
     _close(out, want, bound)
     ops.check_status(eng.device)
+
+
+def test_selections_are_the_callers_own(built_lib):
+    """A later selection, of another layer, another query or on another stream at the same time, leaves an earlier one as it is."""
+    from mserve_b200 import ops
+    from mserve_b200.kv8_cache import PagedKV8
+    B, Hq, H, D, layers = 2, 8, 2, 128, 4
+    g = torch.Generator().manual_seed(3)
+    eng = PagedKV8(layers, B, Hq, H, D, 2000, top_blocks=5)
+    eng.begin_step([2000, 700])
+    for layer in range(layers):
+        k, v = (torch.randn(B, H, 2000, D, generator=g).to(torch.bfloat16).cuda() for _ in range(2))
+        eng.append_layer(layer, k, v)
+    qs = torch.randn(layers, B, Hq, D, generator=g).to(torch.bfloat16).cuda()
+    want = [[t.clone() for t in eng.select(layer, qs[layer])] for layer in range(layers)]
+    assert not torch.equal(want[0][0], want[1][0])
+    held = [eng.select(layer, qs[layer]) for layer in range(layers)]
+    eng.select(0, qs[1])
+    for a, b in zip(held, want):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    streams = [torch.cuda.Stream() for _ in range(layers)]
+    torch.cuda.synchronize()
+    both = []
+    for _ in range(10):
+        for layer, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                both.append((layer, eng.select(layer, qs[layer])))
+    torch.cuda.synchronize()
+    for layer, (idx, counts) in both:
+        assert torch.equal(idx, want[layer][0]) and torch.equal(counts, want[layer][1])
+    ops.check_status(eng.device)
