@@ -57,9 +57,7 @@ class PagedKV8:
         # the step's state on the device: lengths before it, tokens it appends, lengths and blocks after it
         self._state = torch.zeros(4, batch, dtype=torch.int32, device=self.device)
         self.tok0, self.n_new, self.lens, self.held = self._state.unbind(0)
-        self._stage = torch.zeros(4, batch, dtype=torch.int32).pin_memory()
-        self._pt_stage = torch.empty(batch, self.max_pages, dtype=torch.int32).pin_memory()
-        self._stage_ev: Optional[torch.cuda.Event] = None
+        self._most_new = 0                          # tokens that the step appends to one sequence, at most
         self._idx = self._counts = None             # of the last selection, for inspection
 
     # ------------------------------------------------------------------ lengths and pages
@@ -67,9 +65,10 @@ class PagedKV8:
         """Room for n_new tokens of every sequence (an int, or one number each; 0 leaves a sequence as it is).
 
         Maps the pages they need and sets the device-side lengths, through pinned staging copies on the current
-        stream (the host waits only for the previous step's).  append_layer then writes each layer's rows
-        and decode_layer attends over the grown cache.
+        stream; the host waits for nothing.  append_layer then writes each layer's rows and decode_layer attends
+        over the grown cache.  Not to be captured (a replay would send the captured step's lengths again).
         """
+        self._not_captured()
         n_new = np.broadcast_to(np.asarray(n_new, dtype=np.int64), (self.B,))
         if (n_new < 0).any():
             raise ValueError("n_new must not be negative")
@@ -93,6 +92,7 @@ class PagedKV8:
         """
         if not 0 <= b < self.B:
             raise ValueError(f"no sequence {b}")
+        self._not_captured()
         row = self.page_table_h[b]
         self._free.extend(int(p) for p in row[row >= 0])
         row[:] = -1
@@ -100,18 +100,22 @@ class PagedKV8:
         self.len_h[b] = 0
         self._send(self.len_h, np.zeros(self.B, dtype=np.int64), self.len_h, True)
 
+    def _not_captured(self) -> None:
+        with torch.cuda.device(self.device):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("begin_step and reset belong between a captured step's replays, not into the capture")
+
     def _send(self, old: np.ndarray, n_new: np.ndarray, new: np.ndarray, table: bool) -> None:
-        if self._stage_ev is not None:
-            self._stage_ev.synchronize()        # the staging buffers' last copies are done
-        st = self._stage.numpy()
-        st[0], st[1], st[2], st[3] = old, n_new, new, -(-new // self.page_size)
+        self._most_new = int(n_new.max())
+
+        def send(to: torch.Tensor, values: np.ndarray) -> None:
+            # pinned memory of this copy's own: torch's allocator hands it out again when the copy is done
+            to.copy_(torch.from_numpy(values.astype(np.int32)).pin_memory(), non_blocking=True)
+
         with torch.cuda.device(self.device):
             if table:
-                self._pt_stage.numpy()[:] = self.page_table_h
-                self.page_table.copy_(self._pt_stage, non_blocking=True)
-            self._state.copy_(self._stage, non_blocking=True)
-            self._stage_ev = torch.cuda.Event()
-            self._stage_ev.record(torch.cuda.current_stream(self.device))
+                send(self.page_table, self.page_table_h)
+            send(self._state, np.stack([old, n_new, new, -(-new // self.page_size)]))
 
     # ------------------------------------------------------------------ a layer of the step
     def append_layer(self, layer: int, k_new: torch.Tensor, v_new: torch.Tensor) -> None:
@@ -121,8 +125,8 @@ class PagedKV8:
         """
         if k_new.dim() != 4 or k_new.shape[:2] != (self.B, self.Hkv) or k_new.shape[3] != self.D:
             raise ValueError(f"k_new must be [B={self.B}, Hkv={self.Hkv}, n, D={self.D}]")
-        if k_new.shape[2] < int(self._stage[1].max()):
-            raise ValueError(f"the step appends up to {int(self._stage[1].max())} tokens, k_new holds {k_new.shape[2]}")
+        if k_new.shape[2] < self._most_new:
+            raise ValueError(f"the step appends up to {self._most_new} tokens, k_new holds {k_new.shape[2]}")
         ops.kv8_append(self.pages[layer], self.page_table, k_new, v_new, tok0=self.tok0, counts=self.n_new)
 
     def _recent(self, positions: int) -> int:

@@ -1,7 +1,6 @@
 """PagedKV8's host side without a GPU: the calls that a step makes, on stand-ins for the operators."""
 import contextlib
 
-import numpy as np
 import pytest
 import torch
 
@@ -11,7 +10,7 @@ def engine(monkeypatch, built_lib):
     """make(...): a PagedKV8 on CPU tensors whose operator calls are recorded in make.calls as (name, device that is
     current, arguments)."""
     from mserve_b200 import kv8_cache, ops
-    calls, current = [], [None]
+    calls, current, pinned, capturing = [], [None], [], [False]
 
     @contextlib.contextmanager
     def on(device):
@@ -31,7 +30,8 @@ def engine(monkeypatch, built_lib):
                 torch.zeros(n, dtype=torch.int32) if counts is None else counts)
 
     monkeypatch.setattr(torch.cuda, "device", on)
-    monkeypatch.setattr(torch.Tensor, "pin_memory", lambda t, *a: t)
+    monkeypatch.setattr(torch.Tensor, "pin_memory", lambda t, *a: pinned.append(t) or t)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
     monkeypatch.setattr(ops, "kv8_append", record("append"))
     monkeypatch.setattr(ops, "kv8_block_score", record("score"))
     monkeypatch.setattr(ops, "topk", record("topk", topk))
@@ -39,7 +39,7 @@ def engine(monkeypatch, built_lib):
 
     def make(*args, **kw):
         return kv8_cache.PagedKV8(*args, device=torch.device("cpu"), **kw)
-    make.calls = calls
+    make.calls, make.pinned, make.capturing = calls, pinned, capturing
     return make
 
 
@@ -80,3 +80,34 @@ def test_selections_share_nothing(engine):
         assert len({t.data_ptr() for t in tensors}) == 3
     assert [c[2][0].data_ptr() for c in engine.calls if c[0] == "topk"] == [t.data_ptr() for t in scores]
     assert held[0][0].shape == (2, 2, 4) and held[0][1].shape == (2, 2)
+
+
+def test_staging_is_of_each_send(engine):
+    """Every send stages through memory of its own that nothing writes again: earlier copies may still be under way."""
+    eng = engine(1, 2, 4, 2, 64, 1000)
+    engine.pinned.clear()
+    eng.begin_step([17, 3])
+    eng.begin_step([0, 2])
+    eng.reset(0)
+    eng.begin_step(1)
+    states = [t for t in engine.pinned if t.shape == (4, 2)]
+    tables = [t for t in engine.pinned if t.shape == (2, 63)]
+    assert len({t.data_ptr() for t in engine.pinned}) == len(engine.pinned) == len(states) + len(tables)
+    assert [s.tolist() for s in states] == [[[0, 0], [17, 3], [17, 3], [2, 1]], [[17, 3], [0, 2], [17, 5], [2, 1]],
+                                            [[0, 5], [0, 0], [0, 5], [0, 1]], [[0, 5], [1, 1], [1, 6], [1, 1]]]
+    assert [(t >= 0).sum(dim=1).tolist() for t in tables] == [[2, 1], [0, 1], [1, 1]]
+    assert eng.page_table.tolist() == eng.page_table_h.tolist()
+
+
+def test_steps_are_not_captured(engine):
+    eng = engine(1, 2, 4, 2, 64, 1000)
+    eng.begin_step([17, 3])
+    engine.capturing[0] = True
+    for call in (eng.begin_step, lambda: eng.reset(1)):
+        with pytest.raises(RuntimeError, match="captur"):
+            call()
+    engine.capturing[0] = False
+    assert eng.len_h.tolist() == [17, 3] and eng.page_table_h[1, 0] >= 0
+    eng.append_layer(0, torch.zeros(2, 2, 17, 64), torch.zeros(2, 2, 17, 64))
+    with pytest.raises(ValueError, match="up to 17"):
+        eng.append_layer(0, torch.zeros(2, 2, 16, 64), torch.zeros(2, 2, 16, 64))

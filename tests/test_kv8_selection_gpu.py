@@ -72,3 +72,49 @@ def test_selections_are_the_callers_own(built_lib):
     for layer, (idx, counts) in both:
         assert torch.equal(idx, want[layer][0]) and torch.equal(counts, want[layer][1])
     ops.check_status(eng.device)
+
+
+def test_steps_do_not_wait_for_the_device(built_lib):
+    """reset and begin_step return while earlier work of the stream still runs, and each sends its own lengths."""
+    from mserve_b200 import ops
+    from mserve_b200.kv8_cache import PagedKV8
+    eng = PagedKV8(1, 3, 4, 2, 64, 100)
+    for _ in range(6):                              # the staging memory exists
+        eng.begin_step(1)
+        eng.reset(0)
+    eng.reset(1), eng.reset(2)
+    torch.cuda.synchronize()
+    torch.cuda._sleep(400_000_000)                  # a fifth of a second
+    busy = torch.cuda.Event()
+    busy.record()
+    eng.begin_step([20, 5, 0])
+    seen = [(eng.lens.clone(), eng.tok0.clone(), eng.held.clone(), eng.page_table.clone(), eng.page_table_h.copy())]
+    for call in (lambda: eng.begin_step(1), lambda: eng.reset(0), lambda: eng.begin_step([40, 0, 1])):
+        call()
+        seen.append((eng.lens.clone(), eng.tok0.clone(), eng.held.clone(), eng.page_table.clone(), eng.page_table_h.copy()))
+    assert not busy.query(), "a call waited for the stream"
+    torch.cuda.synchronize()
+    assert [s[0].tolist() for s in seen] == [[20, 5, 0], [21, 6, 1], [0, 6, 1], [40, 6, 2]]
+    assert [s[1].tolist() for s in seen] == [[0, 0, 0], [20, 5, 0], [0, 6, 1], [0, 6, 1]]
+    assert [s[2].tolist() for s in seen] == [[2, 1, 0], [2, 1, 1], [0, 1, 1], [3, 1, 1]]
+    for s in seen:
+        assert s[3].tolist() == s[4].tolist()
+    ops.check_status(eng.device)
+
+
+def test_begin_step_in_a_capture_is_refused(built_lib):
+    from mserve_b200.kv8_cache import PagedKV8
+    eng = PagedKV8(1, 1, 4, 2, 64, 100)
+    eng.begin_step(3)
+    x = torch.zeros(4, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        x += 1
+        for call in (eng.begin_step, lambda: eng.reset(0)):
+            with pytest.raises(RuntimeError, match="captur"):
+                call()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert x.tolist() == [1] * 4 and eng.len_h.tolist() == [3] and eng.lens.tolist() == [3]
+    del graph
