@@ -101,7 +101,7 @@ class PagedKV8:
         self._send(self.len_h, np.zeros(self.B, dtype=np.int64), self.len_h, True)
 
     def _not_captured(self) -> None:
-        with torch.cuda.device(self.device):
+        with torch.cuda.device(self.device.index):
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("begin_step and reset belong between a captured step's replays, not into the capture")
 
@@ -112,7 +112,7 @@ class PagedKV8:
             # pinned memory of this copy's own: torch's allocator hands it out again when the copy is done
             to.copy_(torch.from_numpy(values.astype(np.int32)).pin_memory(), non_blocking=True)
 
-        with torch.cuda.device(self.device):
+        with torch.cuda.device(self.device.index):
             if table:
                 send(self.page_table, self.page_table_h)
             send(self._state, np.stack([old, n_new, new, -(-new // self.page_size)]))
@@ -140,12 +140,15 @@ class PagedKV8:
         positions' own tokens can lie in (two, where Q > 1) if that is more, so every position attends to itself.
         """
         recent = self._recent(q.shape[2] if q.dim() == 4 else 1)
-        scores = torch.empty(self.B, self.Hkv, self.max_pages, dtype=torch.float32, device=self.device)
-        ops.kv8_block_score(q, self.pages[layer], self.page_table, lens=self.lens, max_blocks=self.max_pages, out=scores)
-        with torch.cuda.device(self.device):        # ops.topk launches on the current device
-            self._idx, self._counts = ops.topk(scores.view(self.B * self.Hkv, self.max_pages), top_k=self.top_blocks,
-                                               recent=recent, len_=self.held, len_scalar=self.max_pages,
-                                               sel_per_batch=self.Hkv)
+        rows, dev = self.B * self.Hkv, self.device
+        scores = torch.empty(rows, self.max_pages, dtype=torch.float32, device=dev)
+        self._idx = torch.empty(rows, self.top_blocks + recent, dtype=torch.int32, device=dev)
+        self._counts = torch.empty(rows, dtype=torch.int32, device=dev)
+        ops.kv8_block_score(q, self.pages[layer], self.page_table, lens=self.lens, max_blocks=self.max_pages,
+                            out=scores.view(self.B, self.Hkv, self.max_pages))
+        with torch.cuda.device(dev.index):          # ops.topk launches on the current device
+            ops.topk(scores, top_k=self.top_blocks, recent=recent, len_=self.held, len_scalar=self.max_pages,
+                     sel_per_batch=self.Hkv, out=self._idx, counts=self._counts)
         return self._idx.view(self.B, self.Hkv, -1), self._counts.view(self.B, self.Hkv)
 
     def decode_layer(self, layer: int, q: torch.Tensor, *, out: Optional[torch.Tensor] = None,

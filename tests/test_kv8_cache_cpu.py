@@ -46,9 +46,10 @@ def engine(monkeypatch, built_lib):
 def test_selection_runs_on_the_caches_device(engine):
     """The top-k call, which launches on the current device, is made with the cache's device current."""
     eng = engine(1, 2, 4, 2, 64, 100, top_blocks=2)
+    eng.device = torch.device("cpu", 3)
     eng.decode_layer(0, torch.zeros(2, 4, 64, dtype=torch.bfloat16))
     assert [c[0] for c in engine.calls] == ["score", "topk", "attention"]
-    assert engine.calls[1][1] == eng.device
+    assert engine.calls[1][1] == eng.device.index == 3
 
 
 @pytest.mark.parametrize("page", [16, 32, 128])
