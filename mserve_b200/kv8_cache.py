@@ -156,11 +156,13 @@ class PagedKV8:
         """Attention of the last Q tokens over one layer's cache: q [B, Hq, Q, D] (or [B, Hq, D]) -> [B, Hq, Q, D].
 
         Position i of a sequence of length n sees the tokens below n - Q + 1 + i.  t_bound: the length bound
-        that the kernel is launched for (default: the capacity, which stays valid in a captured step while the
-        cache grows).
+        that the kernel is launched for, from the longest sequence's length to the capacity (the default, which
+        stays valid in a captured step while the cache grows; a smaller one does up to that length).
         """
         if q.dim() == 3:
             q = q.unsqueeze(2)
+        if t_bound is not None and not int(self.len_h.max()) <= t_bound <= self.C:
+            raise ValueError(f"t_bound {t_bound} must lie in [{int(self.len_h.max())}, {self.C}]")
         if self.top_blocks:
             idx, counts = self.select(layer, q)
             return ops.kv8_attention(q, self.pages[layer], self.page_table, lens=self.lens, blocks=idx, counts=counts, out=out)

@@ -112,3 +112,19 @@ def test_steps_are_not_captured(engine):
     eng.append_layer(0, torch.zeros(2, 2, 17, 64), torch.zeros(2, 2, 17, 64))
     with pytest.raises(ValueError, match="up to 17"):
         eng.append_layer(0, torch.zeros(2, 2, 16, 64), torch.zeros(2, 2, 16, 64))
+
+
+@pytest.mark.parametrize("top", [0, 2])
+def test_t_bound_covers_the_lengths(engine, top):
+    """A bound below a sequence's length would leave tokens out, and shift what each position sees: refused."""
+    eng = engine(1, 2, 4, 2, 64, 100, top_blocks=top)
+    eng.begin_step([40, 7])
+    q = torch.zeros(2, 4, 1, 64, dtype=torch.bfloat16)
+    for bad in (39, 0, -1, 101, 112):
+        with pytest.raises(ValueError, match="t_bound"):
+            eng.decode_layer(0, q, t_bound=bad)
+    assert not engine.calls
+    for good in (40, 77, 100, None):
+        eng.decode_layer(0, q, t_bound=good)
+    if not top:
+        assert [c[3]["max_tokens"] for c in engine.calls] == [40, 77, 100, 100]
