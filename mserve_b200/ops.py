@@ -605,6 +605,13 @@ def _kv8_status(t: torch.Tensor) -> Optional[torch.Tensor]:
     return w if w is not None else status_word(t.device)
 
 
+def _kv8_on(stream: torch.cuda.Stream, t: torch.Tensor):
+    """The context of a call on `stream`, whose outputs and workspace then belong to it."""
+    if stream.device != t.device:
+        raise ValueError(f"a stream of {stream.device} cannot run a call on tensors of {t.device}")
+    return torch.cuda.stream(stream)
+
+
 def kv8_append(pages: Kv8Pages, page_table: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, *,
                tok0: torch.Tensor, counts: Optional[torch.Tensor] = None, status: bool = True,
                stream: Optional[torch.cuda.Stream] = None) -> None:
@@ -618,7 +625,7 @@ def kv8_append(pages: Kv8Pages, page_table: torch.Tensor, k_new: torch.Tensor, v
     caller's: the next call's tok0, and `lens` of the calls below.
     """
     if stream is not None:
-        with torch.cuda.stream(stream):
+        with _kv8_on(stream, k_new):
             return kv8_append(pages, page_table, k_new, v_new, tok0=tok0, counts=counts, status=status)
     check(_kv8_ext().append(*pages, page_table, k_new, v_new, tok0, counts, _kv8_status(k_new) if status else None))
 
@@ -635,7 +642,7 @@ def kv8_block_score(q: torch.Tensor, pages: Kv8Pages, page_table: torch.Tensor, 
     the last blocks) gives the list for kv8_attention.
     """
     if stream is not None:
-        with torch.cuda.stream(stream):
+        with _kv8_on(stream, q):
             return kv8_block_score(q, pages, page_table, lens=lens, max_blocks=max_blocks, out=out)
     check(_kv8_ext().block_score(q, *pages, page_table, lens, max_blocks, out, _kv8_status(q)))
     return out
@@ -655,7 +662,7 @@ def kv8_attention(q: torch.Tensor, pages: Kv8Pages, page_table: torch.Tensor, *,
     scale: 1/sqrt(D) by default.  Returns [B, Hq, Q, D] in q's dtype.
     """
     if stream is not None:
-        with torch.cuda.stream(stream):     # outputs and workspace belong to the launching stream
+        with _kv8_on(stream, q):
             return kv8_attention(q, pages, page_table, lens=lens, max_tokens=max_tokens, blocks=blocks, counts=counts,
                                  scale=scale, out=out)
     rc, out = _kv8_ext().attention(q, *pages, page_table, lens, max_tokens, blocks, counts, scale, out, _kv8_status(q))
