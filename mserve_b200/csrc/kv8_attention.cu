@@ -7,15 +7,18 @@
 // Mathematics.  Work unit: a tile of 16 tokens, which lies in one page, so both scales are one
 // number.  With base-2 logarithms and t' = s * log2(e) + eV, the second product's weights
 // P = 2^(t' - m) carry V's scale (m: running reference of t' over the tiles), the codes v8 enter it
-// unscaled, and the softmax denominator is sum P * 2^-eV.  Exponents within [-60, 60] keep
-// the term of the largest s above 2^-121 and so in fp32's normal range.  m moves only when a t'
-// exceeds it by more than 8 (then P <= 2^8 until the next move): most tiles need one vote
+// unscaled, and the softmax denominator is sum P * 2^-eV in fp32.  Exponents within [-60, 60] keep
+// its term of the largest s above 2^-121 and so in fp32's normal range.  m moves only when a t'
+// exceeds it by more than 15 (then P <= 2^15 until the next move): most tiles need one vote
 // instead of a maximum over the warp.
 // q is scaled per row to a largest magnitude in [1, 2) and enters as fp16 (a bf16 or fp16 value
 // keeps all its bits down to 2^-14 of the row's largest; below, it is off by at most 2^-25 of that).
 // K and V codes are exact in fp16.  P is rounded to fp16 (relative 2^-11); for fp16 outputs
 // its remainder enters as a second fp16 term, as one term alone would be as far off as the output's
-// own rounding.  All sums are fp32.
+// own rounding.  All sums are fp32.  m starts 7 below the largest t' and so uses fp16's range above 1: the steps of 2^-24
+// at its lower end put a weight off by at most 2^-32 of the largest P of its warp, relative to P by more
+// than the roundings above only where P is below 2^-21 of that -- a score 15 lower, or a page whose V exponent
+// is 21 below another's (one outlier of V raises its page's).  From 2^-32 on a weight counts in the denominator only.
 //
 // Bound by the codes' bytes (2D a token and KV head).  mma.sync m16n8k16 with the tokens on M:
 // S^T = K Q^T, O^T = V^T P^T, so the 8 columns hold the query rows (16 rows: two column tiles, and
@@ -83,6 +86,7 @@ __host__ __device__ constexpr int ka_stages(int d, int nt) { return d == 64 ? (n
 __host__ __device__ constexpr int ka_ctas(int d, int nt) { return d == 256 || (d == 128 && nt == 2) ? 1 : d == 64 && nt == 1 ? 3 : 2; }
 constexpr int kKaMaxCluster = 8;
 constexpr float kNoMax = -3e38f;   // below every finite score's exponent
+constexpr float kBelow = 7.f, kAbove = 15.f;   // m is set 7 below the largest exponent, and again for one over 15 above m
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -445,7 +449,7 @@ struct Kv8Attn {
           if (tok + row + (k >> 1) * 8 >= sm.lim[nt * 8 + 2 * (lane & 3) + (k & 1)]) s[nt][k] = -INFINITY;
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) over |= s[nt][k] > m[nt][k & 1] + 8.f;
+      for (int k = 0; k < 4; ++k) over |= s[nt][k] > m[nt][k & 1] + kAbove;
     }
     if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
@@ -456,7 +460,7 @@ struct Kv8Attn {
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          x = fmaxf(x, m[nt][k]);
+          x = fmaxf(x - kBelow, m[nt][k]);
           const float down = exp2_fast(m[nt][k] - x);
           m[nt][k] = x;
           l[nt][k] *= down;
