@@ -79,9 +79,6 @@ struct Divisor {
 // 2^e for e in [-126, 127].
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-// floor(log2 a) of a finite a > 0 (fp32 subnormals count as 2^-127).
-__device__ __forceinline__ int exponent_of(float a) { return (int)(__float_as_uint(a) >> 23) - 127; }
-
 // The four codes of a word as two half2 (exact): lo = codes 0, 1; hi = codes 2, 3.  An e5m2 code is
 // the upper byte of an fp16, so its conversion is a byte permutation.
 template <bool E5M2>
