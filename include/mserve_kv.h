@@ -370,7 +370,8 @@ int mskv_image_filter(const mskv_filter_desc* d, void* stream);
  *   same 8-bit type, at bounds + ((page*kv_heads + h)*2 + i)*head_dim + d
  * Token t of sequence b is row t % page_size of page page_table[b*pt_stride_b + t/page_size].
  * Requirements: page_size a multiple of 16, <= 128; head_dim 64, 128 or 256; k, v and bounds
- * 16-byte aligned, stride_page and stride_h multiples of 16 bytes.                           */
+ * 16-byte aligned, stride_page and stride_h multiples of 16 bytes, exps 2-byte aligned; in these calls
+ * every array of 32-bit words (page_table, lens, counts, lists, scores, status) 4-byte aligned. */
 #define MSKV_KV8_EXP_MIN (-60)
 #define MSKV_KV8_EXP_MAX 60
 #define MSKV_KV8_MAX_QLEN 16

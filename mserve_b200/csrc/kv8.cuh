@@ -51,6 +51,13 @@ inline int check_kv8(const mskv_kv8_pages& p, const char* what) {
   return MSKV_OK;
 }
 
+// The call's arrays of 32-bit words (lengths, counts, lists, scores, the status word), NULL or aligned.
+template <typename... T>
+inline int check_words(const char* what, const T*... words) {
+  if ((0 | ... | (uintptr_t)words) & 3) return fail(MSKV_ERR_ARG, "%s: arrays of 32-bit words must be 4-byte aligned", what);
+  return MSKV_OK;
+}
+
 // Multiprocessors of the current device, asked for once per device (two plans a call).
 inline int sms_of_device() {
   static std::atomic<int> known[64];

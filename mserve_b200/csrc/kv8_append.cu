@@ -460,6 +460,7 @@ extern "C" int mskv_kv8_append(const mskv_kv8_append_desc* d, void* stream) {
   if (d->num_tokens < 0) return fail(MSKV_ERR_ARG, "mskv_kv8_append: negative num_tokens");
   if (d->num_tokens == 0) return MSKV_OK;
   if (!d->k_new || !d->v_new || !d->tok0) return fail(MSKV_ERR_ARG, "mskv_kv8_append: NULL k_new, v_new or tok0");
+  if (const int rc = check_words("mskv_kv8_append", d->tok0, d->counts, d->status)) return rc;
   const int elem = d->dtype == MSKV_DT_F32 ? 4 : 2;
   const uintptr_t k_bits = (uintptr_t)d->k_new | (uintptr_t)d->k_stride_b | (uintptr_t)d->k_stride_h | (uintptr_t)d->k_stride_t;
   const uintptr_t v_bits = (uintptr_t)d->v_new | (uintptr_t)d->v_stride_b | (uintptr_t)d->v_stride_h | (uintptr_t)d->v_stride_t;

@@ -1210,6 +1210,7 @@ extern "C" int32_t mskv_kv8_expire_waits(int32_t on) { return g_expire.exchange(
 extern "C" int mskv_kv8_attention(const mskv_kv8_attn_desc* d, void* stream) {
   if (const int rc = check_attn(d)) return rc;
   if (!d->q || !d->out || !d->lens) return fail(MSKV_ERR_ARG, "mskv_kv8_attention: NULL q, out or lens");
+  if (const int rc = check_words("mskv_kv8_attention", d->lens, d->blocks, d->counts, d->status)) return rc;
   const uintptr_t q_bits = (uintptr_t)d->q | (uintptr_t)d->q_stride_b | (uintptr_t)d->q_stride_h | (uintptr_t)d->q_stride_q;
   const uintptr_t o_bits = (uintptr_t)d->out | (uintptr_t)d->out_stride_b | (uintptr_t)d->out_stride_h | (uintptr_t)d->out_stride_q;
   if ((q_bits | o_bits) & 1) return fail(MSKV_ERR_ARG, "mskv_kv8_attention: q and out must be aligned to their elements");

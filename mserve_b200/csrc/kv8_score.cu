@@ -188,6 +188,7 @@ extern "C" int mskv_kv8_block_score(const mskv_kv8_score_desc* d, void* stream) 
     return fail(MSKV_ERR_DTYPE, "mskv_kv8_block_score: q must be bf16 or f16");
   if (!d->pages.bounds) return fail(MSKV_ERR_ARG, "mskv_kv8_block_score: the cache has no bounds");
   if (!d->q || !d->lens || !d->scores) return fail(MSKV_ERR_ARG, "mskv_kv8_block_score: NULL q, lens or scores");
+  if (const int rc = check_words("mskv_kv8_block_score", d->lens, d->scores, d->status)) return rc;
   if (d->q_heads <= 0 || d->q_heads % d->pages.kv_heads)
     return fail(MSKV_ERR_ARG, "mskv_kv8_block_score: q_heads must be a multiple of kv_heads");
   if (d->max_blocks < 0 || d->max_blocks > d->pages.max_pages || d->max_blocks > d->scores_stride)

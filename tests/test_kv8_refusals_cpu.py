@@ -17,3 +17,20 @@ def test_streams_of_another_device(ext, monkeypatch):  # noqa: F811
         with pytest.raises(ValueError, match="stream of cuda:1"):
             call(stream=SimpleNamespace(device=torch.device("cuda", 1)))
     assert not entered
+
+
+def test_c_refuses_unaligned_words(built_lib):
+    """Lengths, counts, lists, scores and the status word at addresses that a 32-bit access would fault on."""
+    import ctypes as C
+    from mserve_b200 import _lib
+    from test_kv8_cpu import _append, _attn, _score
+    lib = _lib.lib()
+    for make, fn, names in ((_append, lib.mskv_kv8_append, ("tok0", "counts", "status")),
+                            (_score, lib.mskv_kv8_block_score, ("lens", "scores", "status")),
+                            (_attn, lib.mskv_kv8_attention, ("lens", "blocks", "counts", "status"))):
+        for name in names:
+            for off in (1, 2, 3):
+                d = make()
+                setattr(d, name, (20 << 20) + off)
+                assert fn(C.byref(d), None) == _lib.MSKV_ERR_ARG, (fn, name)
+                assert b"aligned" in lib.mskv_last_error()
