@@ -99,6 +99,12 @@ void same_device(const c10::Device& d, const OptTensor& t) {
   if (t && t->device() != d) bad_value("all tensors of the call must live on " + d.str());
 }
 
+// Outputs whose rows lie on each other (expanded ones) would be written by several blocks at once.
+void no_overlap(const at::Tensor& t, const char* name) {
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1 && t.stride(i) == 0) bad_value(std::string(name) + " must not be expanded: its elements share memory");
+}
+
 uint32_t* status_ptr(const OptTensor& t) { return t ? reinterpret_cast<uint32_t*>(t->data_ptr()) : nullptr; }
 
 int append(const at::Tensor& k, const at::Tensor& v, const at::Tensor& exps, const OptTensor& bounds, const at::Tensor& table,
@@ -115,6 +121,7 @@ int append(const at::Tensor& k, const at::Tensor& v, const at::Tensor& exps, con
   if (H != k.size(1) || D != k.size(3)) bad_value("rows " + shape_text(k_new) + " do not match a cache of " + shape_text(k));
   if (n && (k_new.stride(3) != 1 || v_new.stride(3) != 1)) bad_value("the head_dim axis of the rows must be contiguous");
   if (n > INT32_MAX) bad_value("too many rows for one call");
+  for (const at::Tensor* pool : {&k, &v}) no_overlap(*pool, "a cache that is appended to");
   d.tok0 = int32_list(tok0, B, "tok0");
   if (counts) d.counts = int32_list(*counts, B, "counts");
   const c10::Device dev = one_device("k_new", k_new, v_new, k, v, exps, table, tok0);
@@ -152,6 +159,7 @@ int block_score(const at::Tensor& q_in, const at::Tensor& k, const at::Tensor& v
   if (out.scalar_type() != at::kFloat || out.dim() != 3 || out.size(0) != B || out.size(1) != H || out.size(2) < max_blocks ||
       (out.size(2) > 1 && out.stride(2) != 1) || (B > 1 && H > 1 && out.stride(0) != H * out.stride(1)))
     bad_value("out must be fp32 [B, Hkv, >= max_blocks] with rows at a common stride");
+  no_overlap(out, "out");
   if (max_blocks < 0 || max_blocks > table.size(1)) bad_value("max_blocks must lie in [0, " + std::to_string(table.size(1)) + "]");
   d.lens = int32_list(lens, B, "lens");
   const c10::Device dev = one_device("q", q_in, k, v, exps, *bounds, table, lens, out);
@@ -204,6 +212,7 @@ std::tuple<int, at::Tensor> attention(const at::Tensor& q, const at::Tensor& k, 
   }
   if (out_in && (out_in->sizes() != q.sizes() || out_in->scalar_type() != q.scalar_type() || out_in->stride(3) != 1))
     bad_value("out must have q's shape and dtype and a contiguous head_dim");
+  if (out_in) no_overlap(*out_in, "out");
   const c10::Device dev = one_device("q", q, k, v, exps, table, lens);
   same_device(dev, bounds);
   same_device(dev, blocks);

@@ -34,3 +34,19 @@ def test_c_refuses_unaligned_words(built_lib):
                 setattr(d, name, (20 << 20) + off)
                 assert fn(C.byref(d), None) == _lib.MSKV_ERR_ARG, (fn, name)
                 assert b"aligned" in lib.mskv_last_error()
+
+
+def test_expanded_outputs(ext):  # noqa: F811
+    """Outputs whose elements share memory: several blocks would write them at once."""
+    from mserve_b200 import ops
+    pages, table = ops.kv8_pages(4, 2, 128, device="cpu"), torch.zeros(3, 5, dtype=torch.int32)
+    append, score, attend = _calls(pages, table, B=3)
+    one = torch.zeros(1, 1, 1, 128, dtype=torch.bfloat16)
+    for out in (one.expand(3, 6, 1, 128), torch.zeros(3, 1, 1, 128, dtype=torch.bfloat16).expand(3, 6, 1, 128),
+                torch.zeros(1, 6, 1, 128, dtype=torch.bfloat16).expand(3, 6, 1, 128)):
+        with pytest.raises(ValueError, match="expanded"):
+            attend(out=out)
+    with pytest.raises(ValueError, match="must"):
+        score(out=torch.zeros(1, 1, 4).expand(3, 2, 4))
+    with pytest.raises(ValueError, match="expanded"):
+        append(pages=pages._replace(k=pages.k[:1].expand(4, 2, 16, 128), v=pages.v[:1].expand(4, 2, 16, 128)))
