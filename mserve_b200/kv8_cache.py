@@ -34,8 +34,11 @@ class PagedKV8:
     def __init__(self, num_layers: int, batch: int, q_heads: int, kv_heads: int, head_dim: int, capacity: int, *,
                  top_blocks: int = 0, recent_blocks: int = 1, page_size: int = 16,
                  cache_dtype: torch.dtype = torch.float8_e4m3fn, device: Optional[torch.device] = None):
+        if num_layers <= 0:
+            raise ValueError("num_layers must be positive")
         if batch <= 0 or kv_heads <= 0 or q_heads <= 0 or q_heads % kv_heads:
             raise ValueError("q_heads must be a positive multiple of kv_heads, batch positive")
+        ops.check_kv8_layout(page_size, head_dim, cache_dtype)
         if capacity <= 0:
             raise ValueError("capacity must be positive")
         if top_blocks < 0 or (top_blocks > 0 and recent_blocks < 1):
@@ -69,7 +72,10 @@ class PagedKV8:
         over the grown cache.  Not to be captured (a replay would send the captured step's lengths again).
         """
         self._not_captured()
-        n_new = np.broadcast_to(np.asarray(n_new, dtype=np.int64), (self.B,))
+        given = np.asarray(n_new)
+        if given.dtype.kind not in "iu" or given.shape not in ((), (self.B,)):
+            raise ValueError(f"n_new must be an integer or one for each of the {self.B} sequences")
+        n_new = np.broadcast_to(given.astype(np.int64), (self.B,))
         if (n_new < 0).any():
             raise ValueError("n_new must not be negative")
         new_len = self.len_h + n_new

@@ -560,16 +560,21 @@ class Kv8Pages(NamedTuple):
     bounds: Optional[torch.Tensor] = None
 
 
-def kv8_pages(num_pages: int, kv_heads: int, head_dim: int, *, page_size: int = 16,
-              dtype: torch.dtype = torch.float8_e4m3fn, device: Optional[torch.device] = None,
-              bounds: bool = True) -> Kv8Pages:
-    """Zeroed pages of an 8-bit cache (one layer) on `device`."""
+def check_kv8_layout(page_size: int, head_dim: int, dtype: torch.dtype) -> None:
+    """Raises TypeError or ValueError for pages that the 8-bit cache does not have."""
     if dtype not in KV8_DTYPES:
         raise TypeError(f"the 8-bit cache is float8_e4m3fn or float8_e5m2, got {dtype}")
     if page_size <= 0 or page_size % 16 or page_size > 128:
         raise ValueError("page_size must be a multiple of 16, at most 128")
     if head_dim not in (64, 128, 256):
         raise ValueError("head_dim must be 64, 128 or 256")
+
+
+def kv8_pages(num_pages: int, kv_heads: int, head_dim: int, *, page_size: int = 16,
+              dtype: torch.dtype = torch.float8_e4m3fn, device: Optional[torch.device] = None,
+              bounds: bool = True) -> Kv8Pages:
+    """Zeroed pages of an 8-bit cache (one layer) on `device`."""
+    check_kv8_layout(page_size, head_dim, dtype)
     dev = _norm(device if device is not None else "cuda")
 
     def zeros(*shape):

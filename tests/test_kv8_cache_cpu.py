@@ -128,3 +128,21 @@ def test_t_bound_covers_the_lengths(engine, top):
         eng.decode_layer(0, q, t_bound=good)
     if not top:
         assert [c[3]["max_tokens"] for c in engine.calls] == [40, 77, 100, 100]
+
+
+def test_arguments(engine):
+    """Sizes that no cache has are refused as such, token counts that are no integers too: nothing is rounded or divided by."""
+    make = dict(num_layers=1, batch=2, q_heads=4, kv_heads=2, head_dim=64, capacity=64)
+    for kw in (dict(page_size=0), dict(page_size=-16), dict(page_size=24), dict(head_dim=96), dict(num_layers=0)):
+        with pytest.raises(ValueError, match="page_size|head_dim|num_layers"):
+            engine(**{**make, **kw})
+    with pytest.raises(TypeError):
+        engine(**make, cache_dtype=torch.float16)
+    eng = engine(**make)
+    for bad in (1.5, [1.0, 2.0], [1, 2, 3], [[1, 1]], [3], "1"):
+        with pytest.raises(ValueError, match="n_new"):
+            eng.begin_step(bad)
+    assert eng.len_h.tolist() == [0, 0] and (eng.page_table_h < 0).all()
+    for good in (3, [1, 0], (0, 2), torch.tensor([2, 2]), torch.tensor(1)):
+        eng.begin_step(good)
+    assert eng.len_h.tolist() == [7, 8]
