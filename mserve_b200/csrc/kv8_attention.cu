@@ -553,6 +553,17 @@ struct Kv8Attn {
       for (int i = 0; i < kVWords; ++i) vr[r][i] &= ~nonfinite_bytes<E5M2>(vr[r][i]);
   }
 
+  // The bounded wait for the tile at `place` ran out, `left` before the warp's last: the rows are incomplete, so say so, wait
+  // (again with a limit) for the copies still in flight and take no more tiles, of this segment or another: the
+  // CTA contributes nothing from here on.  Kept out of the tile loop's code.
+  static __device__ __noinline__ void give_up(uint32_t* status, Smem& sm, RingPlace<kStages> place, uint32_t bars, int left, int lane) {
+    if (lane == 0) {
+      if (status) atomicOr(status, MSKV_STATUS_TIMEOUT);
+      sm.expired = 1;
+    }
+    place.drain(0, left, [&](int stage, uint32_t phase) { return bulk_wait(bars + 8 * stage, phase); });
+  }
+
   // The CTA's tiles of the segment: the warp's share (every kWarps-th).  The first tile's codes are on their way
   // while the query is staged.
   __device__ __forceinline__ void piece(const Kv8AttnDev& a, const CUtensorMap* k_map, const CUtensorMap* v_map, Smem& sm, const Place& at,
@@ -578,17 +589,8 @@ struct Kv8Attn {
     stage_q(a, sm, q, rt, len, warp, lane);
     __syncthreads();
     start(sm, lane);
-    // The bounded wait for tile i ran out: the rows are incomplete, so say so, wait (again with a limit) for the copies
-    // still in flight and take no more tiles, of this segment or another: the CTA contributes nothing from here on.
-    const auto give_up = [&](int i) {
-      if (lane == 0) {
-        if (a.status) atomicOr(a.status, MSKV_STATUS_TIMEOUT);
-        sm.expired = 1;
-      }
-      place.drain(i, n, [&](int stage, uint32_t phase) { return bulk_wait(bars + 8 * stage, phase); });
-    };
     if (a.expire && n > 0) {
-      give_up(0);
+      give_up(a.status, sm, place, bars, n, lane);
       n = 0;
     }
 #pragma unroll 1
@@ -601,7 +603,7 @@ struct Kv8Attn {
       const int tok = __shfl_sync(0xffffffffu, now.tok, i & 31), exps = __shfl_sync(0xffffffffu, now.exps, i & 31);
       const uint32_t bar = bars + 8 * place.stage, tile = ring + place.stage * kTileBytes;
       if (!__all_sync(0xffffffffu, bulk_wait(bar, place.phase))) {
-        give_up(i);
+        give_up(a.status, sm, place, bars, n - i, lane);
         break;
       }
       if (exps & 0x10000) {

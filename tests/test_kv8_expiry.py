@@ -86,7 +86,7 @@ def test_drain_waits_for_every_load_in_flight(tmp_path):
 def test_kernel_uses_the_ring(built_lib):
     """What is tested above is what the kernel runs: it keeps no stage or phase beside the ring's."""
     source = (CSRC / "kv8_attention.cu").read_text()
-    assert "RingPlace<kStages> place(turn);" in source and "place.drain(i, n," in source
+    assert "RingPlace<kStages> place(turn);" in source and "place.drain(0, left," in source
     assert "% kStages" not in source and "phase ^= 1" not in source and source.count("turn += n;") == 1
 
 
