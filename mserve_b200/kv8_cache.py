@@ -139,12 +139,17 @@ class PagedKV8:
         """Last pages that are always attended: recent_blocks, and those of the last `positions` tokens wherever they end in a page."""
         return max(self.recent_blocks, 1 - (1 - positions) // self.page_size)
 
+    def _check_q(self, q: torch.Tensor) -> None:
+        if q.dim() not in (3, 4) or q.shape[:2] != (self.B, self.Hq) or q.shape[-1] != self.D:
+            raise ValueError(f"q must be [B={self.B}, Hq={self.Hq}, (Q,) D={self.D}], got {list(q.shape)}")
+
     def select(self, layer: int, q: torch.Tensor):
         """Pages for q [B, Hq, D] or [B, Hq, Q, D]: (indices [B, Hkv, top + recent], ascending, counts [B, Hkv]), the caller's own.
 
         The best top_blocks are those of the last position's scores; the last pages are recent_blocks, or as many as the Q
         positions' own tokens can lie in (two, where Q > 1) if that is more, so every position attends to itself.
         """
+        self._check_q(q)
         recent = self._recent(q.shape[2] if q.dim() == 4 else 1)
         rows, dev = self.B * self.Hkv, self.device
         scores = torch.empty(rows, self.max_pages, dtype=torch.float32, device=dev)
@@ -165,6 +170,7 @@ class PagedKV8:
         that the kernel is launched for, from the longest sequence's length to the capacity (the default, which
         stays valid in a captured step while the cache grows; a smaller one does up to that length).
         """
+        self._check_q(q)
         if q.dim() == 3:
             q = q.unsqueeze(2)
         if t_bound is not None and not int(self.len_h.max()) <= t_bound <= self.C:

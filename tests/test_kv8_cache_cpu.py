@@ -146,3 +146,16 @@ def test_arguments(engine):
     for good in (3, [1, 0], (0, 2), torch.tensor([2, 2]), torch.tensor(1)):
         eng.begin_step(good)
     assert eng.len_h.tolist() == [7, 8]
+
+
+@pytest.mark.parametrize("top", [0, 2])
+def test_queries_of_another_model(engine, top):
+    """Query heads that are not the cache's would be grouped otherwise without a word."""
+    eng = engine(1, 2, 4, 2, 64, 100, top_blocks=top)
+    eng.begin_step(5)
+    for shape in ((2, 8, 64), (2, 2, 1, 64), (1, 4, 64), (2, 4, 32), (2, 4), (2, 4, 1, 1, 64)):
+        with pytest.raises(ValueError, match="Hq=4"):
+            eng.decode_layer(0, torch.zeros(shape, dtype=torch.bfloat16))
+        with pytest.raises(ValueError, match="Hq=4"):
+            eng.select(0, torch.zeros(shape, dtype=torch.bfloat16))
+    assert not engine.calls

@@ -118,3 +118,28 @@ def test_begin_step_in_a_capture_is_refused(built_lib):
     torch.cuda.synchronize()
     assert x.tolist() == [1] * 4 and eng.len_h.tolist() == [3] and eng.lens.tolist() == [3]
     del graph
+
+
+def test_more_blocks_than_there_are(built_lib):
+    """top_blocks beyond the pages that a sequence has, or can have: the whole cache; short and empty sequences among them."""
+    from mserve_b200 import ops
+    from mserve_b200.kv8_cache import PagedKV8
+    g = torch.Generator().manual_seed(8)
+    lens = [200, 16, 17, 1, 0]
+    x = torch.randn(2, 5, 2, 200, 64, generator=g).to(torch.bfloat16).cuda()
+    q = torch.randn(5, 6, 3, 64, generator=g).to(torch.bfloat16).cuda()
+    outs = []
+    for top, recent in ((0, 1), (1000, 1), (5, 50), (1, 12)):
+        eng = PagedKV8(1, 5, 6, 2, 64, 200, top_blocks=top, recent_blocks=recent)
+        eng.begin_step(lens)
+        eng.append_layer(0, x[0], x[1])
+        outs.append(eng.decode_layer(0, q))
+        if top:
+            counts = eng.select(0, q)[1].cpu()
+            assert counts.tolist() == [[min(-(-n // 16), top + max(recent, 2))] * 2 for n in lens]
+    # the same tokens in the same order, split otherwise: the sums' rounding, then the output's
+    whole = outs[0].double()
+    for out in outs[1:]:
+        assert ((out.double() - whole).abs() <= 2.0 ** -7 * whole.abs() + 2.0 ** -10).all()
+    assert (whole[4] == 0).all() and (whole[3, :, :2] == 0).all()
+    ops.check_status(torch.device("cuda"))
