@@ -369,6 +369,8 @@ int mskv_image_filter(const mskv_filter_desc* d, void* stream);
  *   bounds: the elementwise minimum (i = 0) and maximum (i = 1) of the page's K codes, in the
  *   same 8-bit type, at bounds + ((page*kv_heads + h)*2 + i)*head_dim + d
  * Token t of sequence b is row t % page_size of page page_table[b*pt_stride_b + t/page_size].
+ * Codes are finite or NaN, as mskv_kv8_append writes them: an infinite e5m2 code from elsewhere counts as the
+ * largest finite one when its page is appended to, and as NaN or infinite in the attention.
  * Requirements: page_size a multiple of 16, <= 128; head_dim 64, 128 or 256; k, v and bounds
  * 16-byte aligned, stride_page and stride_h multiples of 16 bytes, exps 2-byte aligned; in these calls
  * every array of 32-bit words (page_table, lens, counts, lists, scores, status) 4-byte aligned. */

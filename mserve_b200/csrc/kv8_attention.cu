@@ -15,10 +15,13 @@
 // keeps all its bits down to 2^-14 of the row's largest; below, it is off by at most 2^-25 of that).
 // K and V codes are exact in fp16.  P is rounded to fp16 (relative 2^-11); for fp16 outputs
 // its remainder enters as a second fp16 term, as one term alone would be as far off as the output's
-// own rounding.  All sums are fp32.  m starts 7 below the largest t' and so uses fp16's range above 1: the steps of 2^-24
-// at its lower end put a weight off by at most 2^-32 of the largest P of its warp, relative to P by more
-// than the roundings above only where P is below 2^-21 of that -- a score 15 lower, or a page whose V exponent
-// is 21 below another's (one outlier of V raises its page's).  From 2^-32 on a weight counts in the denominator only.
+// own rounding.  For bf16 outputs, whose rounding is eight times as coarse, one term adds 0.5% to the error
+// against 64 bits (1.681e-3 of the 2-norm against 1.673e-3, 8 x 16384 tokens; up to 9% of the values round
+// to another bf16), and the second would cost 4% (16 x 32768 tokens 173 us -> 180) to 11% (two column tiles, 36.7 -> 40.6).
+// All sums are fp32.  m starts 7 below the largest t' and so uses fp16's range above 1: the steps of 2^-24 at its lower
+// end put a weight off by at most 2^-32 of the largest P of its warp, relative to P by more than the roundings above only
+// where P is below 2^-21 of that -- a score 15 lower, or a page whose V exponent is 21 below another's (one
+// outlier of V raises its page's).  From 2^-32 on a weight counts in the denominator only.
 //
 // Bound by the codes' bytes (2D a token and KV head).  mma.sync m16n8k16 with the tokens on M:
 // S^T = K Q^T, O^T = V^T P^T, so the 8 columns hold the query rows (16 rows: two column tiles, and
@@ -32,13 +35,15 @@
 // the legacy pipe is a fifth busy at the memory's speed.
 //
 // Split: a segment is a (sequence, KV head, row tile).  Where the segments fill the GPU evenly, or are short, a
-// thread-block cluster (of one CTA, where they are many) takes each and merges through distributed shared memory.  Otherwise all tiles of all
-// segments form one line, cut into parts for the CTAs however ragged the lengths are (a scan over the
+// thread-block cluster (of one CTA, where they are many) takes each and merges through distributed shared memory.
+// Otherwise all tiles of all segments form one line, cut into parts for the CTAs however ragged the lengths are (a scan over the
 // lengths in every CTA); a segment of several parts goes through the workspace and a second kernel.
 //
 // Measured (device time, three sets of inputs in turn): 40/8 heads, 128 dims, 16 sequences of 32768 tokens
-// (1.07 GB) 173 us = 0.95 of the copy rate; 28/4 heads, 8 of 16384 (134 MB) 28.6 us = 0.72, of which 3 us pass
-// before the first codes are there and 2 after the last; 136 listed pages of each (18 MB) 8.8 us.
+// (1.07 GB) 173 us = 0.95 of the copy rate in a burst, 189 = 0.87 in calls that go on for tenths of a second, at the power
+// limit's clocks; 16/4 heads of 256 dims, the same bytes 172 us, 64/8 heads of 64 dims, half of them, 114 us = 0.72; 28/4
+// heads, 8 of 16384 (134 MB) 28.3 us = 0.73, of which 3 us pass before the first codes are there and 2 after the
+// last; 136 listed pages of each (18 MB) 8.8 us.
 // Loads straight into registers instead of the ring (one tile ahead, as many as the registers hold): 181,
 // 32.5 and 11.7 us, and 10% more than that at the clocks of a GPU at its power limit; the same chunks through
 // cp.async into a ring: 257 us for the first.
@@ -1076,7 +1081,8 @@ static Kv8Plan make_plan(const mskv_kv8_attn_desc& d) {
   // kernel (4 us, and 4 more where parts would cross segments), but the segments wait for the longest: its tiles a
   // warp, at the time that one takes on an SM of its own.  It is chosen while that is less than what the codes take
   // at 6.3 TB/s, as far as the clusters fill the GPU, and those 4 us; of whole caches, whose lengths may differ, 0.85
-  // of the codes' time and 25 us at most are counted (lists are of one length as a rule).  A cluster has two tiles
+  // of the codes' time and 25 us at most are counted (lists are of one length as a rule): past that the line's 4 us are
+  // little beside what uneven lengths cost a cluster (16 of 32768 below, 107 us of codes a cluster).  A cluster has two tiles
   // a warp or fewer where all clusters run at once.  Measured, cluster / line: 28/4 heads, 8 sequences of 16384 tokens
   // 28.0 / 31.6 us (ragged down to an eighth 23.1 / 22.0), 16 of 4096 17.0 / 20.8, 64 of up to 4096 41.2 / 46.1, 4 of
   // 32768 41.0 / 31.7, 5 of up to 9000 14.2 / 11.6; 40/8 heads, 30 of up to 2900 30.3 / 36.4, 16 of 32768 175 / 173, ragged
