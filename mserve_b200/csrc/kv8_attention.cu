@@ -934,15 +934,15 @@ __global__ void __launch_bounds__(kKmWarps * 32) kv8_merge_kernel(const Kv8AttnD
   const int rt = seg % a.row_tiles, bh = seg / a.row_tiles;
   const int b = (int)a.by_heads.quotient(bh), h = bh - b * a.pg.heads;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // the lengths are those that the first kernel, which waited for whatever wrote them, has read already
-  const bool empty = kv8_tiles(a, b, h) == 0;
   wait_for_previous_grid();
   allow_dependents();
+  // both on their way at once; nobody wrote the entry of a segment without tiles, and nothing follows it
+  const int4 info = a.info[seg];
+  const bool empty = kv8_tiles(a, b, h) == 0;
   if (rt * kRows + r >= a.rows) return;
   float top = kNoMax, sum = 0.f;
   float x[kPer] = {};
   if (!empty) {
-    const int4 info = a.info[seg];
     if (info.x == info.y) return;                     // written by its CTA
 #pragma unroll 1
     for (int c0 = info.x + warp; c0 <= info.y; c0 += kKmWarps * kAtOnce) {
