@@ -458,7 +458,8 @@ int mskv_kv8_block_score(const mskv_kv8_score_desc* d, void* stream);
  * (MSKV_STATUS_INDEX_OOB), as are unmapped pages (MSKV_STATUS_BAD_PAGE).  Scores, softmax and
  * sums in fp32; softmax weights times V's scale enter the second product as fp16 (two fp16 terms for
  * fp16 outputs), off by at most 2^-32 of the largest beyond their relative rounding: a V outlier that raises
- * one page's exponent by more than about 20 costs the other pages' values precision.  `workspace` must hold mskv_kv8_attention_workspace_bytes(d) bytes of device memory,
+ * one page's exponent by more than about 20 costs the other pages' values precision.
+ * `workspace` must hold mskv_kv8_attention_workspace_bytes(d) bytes of device memory,
  * 16-byte aligned; every launch writes all it uses of it.  Calls that may overlap must not share one.
  * stride_page and stride_h must lie in (0, 2^40) here (codes are loaded by TMA).  Every wait on such a load
  * is bounded; one that runs out leaves the row incomplete and sets MSKV_STATUS_TIMEOUT (the block that

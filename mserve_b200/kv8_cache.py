@@ -170,7 +170,6 @@ class PagedKV8:
         that the kernel is launched for, from the longest sequence's length to the capacity (the default, which
         stays valid in a captured step while the cache grows; a smaller one does up to that length).
         """
-        self._check_q(q)
         if q.dim() == 3:
             q = q.unsqueeze(2)
         if t_bound is not None and not int(self.len_h.max()) <= t_bound <= self.C:
@@ -178,6 +177,7 @@ class PagedKV8:
         if self.top_blocks:
             idx, counts = self.select(layer, q)
             return ops.kv8_attention(q, self.pages[layer], self.page_table, lens=self.lens, blocks=idx, counts=counts, out=out)
+        self._check_q(q)
         return ops.kv8_attention(q, self.pages[layer], self.page_table, lens=self.lens,
                                  max_tokens=self.C if t_bound is None else t_bound, out=out)
 
