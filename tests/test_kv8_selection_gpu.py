@@ -84,7 +84,7 @@ def test_steps_do_not_wait_for_the_device(built_lib):
         eng.reset(0)
     eng.reset(1), eng.reset(2)
     torch.cuda.synchronize()
-    torch.cuda._sleep(400_000_000)                  # a fifth of a second
+    torch.cuda._sleep(800_000_000)                  # four tenths of a second
     busy = torch.cuda.Event()
     busy.record()
     eng.begin_step([20, 5, 0])
